@@ -14,11 +14,18 @@ Beyond the reference (which is forward-only): ``ring_flash_attn`` is differentia
 ``ring_flash_attn_with_lse`` / ``ring_flash_attn_backward`` run the forward (returning the
 LSE) and the ring backward explicitly.
 
+Also beyond the reference, the serving side of a paged K/V cache (:mod:`fa4_ring.paged_cache`):
+``paged_block_tables``, ``paged_tree_mask``, ``paged_kv_write``, ``paged_kv_accept`` and the
+attention of decode steps and drafted trees, ``b200_attn_paged_tree``.
+
 There is no CPU fallback: every op needs the built CUDA library and CUDA tensors.
 """
 
+from .attn_backend import b200_attn_paged_tree
 from .config import MERGE_MODES, RingConfig
 from .merge import BatchedMerger, IncrementalMerger, make_merger
+from .paged_cache import (PagedPlan, paged_block_tables, paged_kv_accept, paged_kv_write,
+                          paged_tree_mask)
 from .ring_attention import Descales, ring_flash_attn, ring_flash_attn_with_lse
 from .ring_backward import ring_flash_attn_backward
 from .zigzag import zigzag_shard, zigzag_unshard
@@ -34,4 +41,10 @@ __all__ = [
     "make_merger",
     "ring_flash_attn_with_lse",
     "ring_flash_attn_backward",
+    "b200_attn_paged_tree",
+    "PagedPlan",
+    "paged_block_tables",
+    "paged_tree_mask",
+    "paged_kv_write",
+    "paged_kv_accept",
 ]

@@ -8,6 +8,7 @@ reference raises (AssertionError / ValueError for bad arguments,
 failing backend, ``fa4_ring/fa4_backend.py:83-87``).
 """
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -99,8 +100,20 @@ _SIGNATURES = {
                        _i64, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp],
     "fa4cp_convert_f32": [_vp, _vp, _i64, _i32, _vp],
     "fa4cp_add_f32": [_vp, _vp, _i64, _vp],
+    "fa4cp_paged_block_tables": [_vp, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _i64,
+                                 _vp, _vp, _vp, _vp, _vp],
+    "fa4cp_paged_tree_mask": [_vp, _vp, _i32, _i64, _i32, _vp, _vp],
+    "fa4cp_paged_kv_write": [_vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _vp, _i64,
+                             _i32, _i32, _i32, _i32, _vp, _vp, _vp],
+    "fa4cp_paged_kv_accept": [_vp, _vp, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp,
+                              _i32, _i32, _i32, _i32, _vp, _vp],
+    "fa4cp_attn_paged_tree_workspace_bytes": [_i32, _i32, _i32, _i32],
+    "fa4cp_attn_fwd_paged_tree": [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp,
+                                  _vp, _vp, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _i32, _vp,
+                                  _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp],
 }
-_RESTYPE = {"fa4cp_last_error": ctypes.c_char_p, "fa4cp_attn_kv8_workspace_bytes": _i64}
+_RESTYPE = {"fa4cp_last_error": ctypes.c_char_p, "fa4cp_attn_kv8_workspace_bytes": _i64,
+            "fa4cp_attn_paged_tree_workspace_bytes": _i64}
 
 EXPORTED = tuple(_SIGNATURES)
 
@@ -168,6 +181,14 @@ def dtype_code(dt: torch.dtype) -> int:
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_no_switch = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """Context in which launches go to ``dev`` (nothing to do when it is the current device)."""
+    return _no_switch if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def ptr(t) -> int:

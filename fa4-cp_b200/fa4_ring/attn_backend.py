@@ -12,6 +12,7 @@ accumulators, TMA tiles); FP8 e4m3 inputs produce a bf16 output.
 one of the three zig-zag step patterns, addressing the row halves in place.
 """
 
+import ctypes
 import math
 from typing import Optional, Tuple
 
@@ -226,5 +227,112 @@ def b200_attn_paged(
         1 if causal else 0, float(softmax_scale), _lib.ptr(qd), _lib.ptr(kd), _lib.ptr(vd),
         _lib.stream_of(q))
     _lib.check(rc, "attn_fwd_paged")
+    _lib.count_launches()
+    return out, lse
+
+
+_Strides = ctypes.c_int64 * 3
+
+
+def pool_strides(pool: torch.Tensor, what: str):
+    """(page, row, head) strides, in elements, of a pool ``[pages, page, H_kv, D]``.  Any view
+    with a dense last dimension is taken as it is; the library wants the strides in multiples
+    of 16 bytes.  (A pool is never copied: a copy would double the cache, and a write into it
+    would be lost.)"""
+    n, rows, heads, d = pool.shape
+    sp, sr, sh, sd = pool.stride()
+    if sd != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    return _Strides(sp if n > 1 else rows * heads * d, sr if rows > 1 else heads * d,
+                    sh if heads > 1 else d)
+
+
+def rows16(x: torch.Tensor) -> torch.Tensor:
+    """``x [T, H, D]`` as rows of ``H * D`` dense elements at a 16-byte aligned token stride:
+    a slice of a fused projection is taken as it is, anything else is copied."""
+    _, heads, d = x.shape
+    if (x.stride(2) == 1 and (heads == 1 or x.stride(1) == d)
+            and x.stride(0) * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0):
+        return x
+    return x.contiguous()
+
+
+def as_i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
+        return t
+    return t.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def b200_attn_paged_tree(
+    q: torch.Tensor,            # [T, H, D]
+    k_pages: torch.Tensor,      # [num_pages, page_size, H_kv, D]
+    v_pages: torch.Tensor,      # [num_pages, page_size, H_kv, D]
+    block_table: torch.Tensor,  # int32 [num_seqs, max_pages_per_seq]
+    *,
+    cu_seqlens_q: torch.Tensor,  # int32 [num_seqs + 1]
+    seq_lens: torch.Tensor,      # int32 [num_seqs], cached tokens, the step's own included
+    max_seqlen_q: int,
+    tree_mask: Optional[torch.Tensor] = None,  # int64 [T, words]
+    softmax_scale: Optional[float] = None,
+    q_descale: Optional[torch.Tensor] = None,
+    k_descale: Optional[torch.Tensor] = None,
+    v_descale: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Attention of a few new tokens a request over its paged K/V cache
+    (``fa4cp_attn_fwd_paged_tree``): decode steps and the verification of drafted trees.
+
+    Request ``j`` brings the tokens ``cu_seqlens_q[j] .. cu_seqlens_q[j + 1]``; their K/V are
+    the last rows of its ``seq_lens[j]`` cached tokens (see
+    :mod:`fa4_ring.paged_cache`).  Every token sees all rows before them, and of the new rows
+    those that its ``tree_mask`` bits name (:func:`fa4_ring.paged_tree_mask`): bit ``m`` of
+    word ``w`` is node ``64 w + m`` of its request.  Without a mask a token sees the new rows
+    up to its own (bottom-right causal, as :func:`b200_attn`); one token a request is decode.
+
+    q is f16 / bf16 with K/V of its dtype, or f16 / bf16 / e4m3 with e4m3 K/V (and their
+    descales, scalar, ``[H_kv]`` or ``(1, H_kv)``); head_dim 64, 128 or 256; page_size 16, 32,
+    64 or a multiple of 128.  The pools may be views of another layout.  Long caches are split
+    over the GPU whatever the batch.  Returns ``(out [T, H, D], lse [T, H] fp32 natural log)``;
+    out has q's dtype (bf16 for e4m3).  A row that sees no key gets out 0, lse -inf.  What lies
+    behind ``seq_lens`` in a page never reaches the result, nor does what a token does not see.
+    Rows outside ``cu_seqlens_q`` are left unwritten."""
+    _lib.require_cuda(q, k_pages, v_pages, block_table, tree_mask)
+    assert q.dim() == 3, "expected a [T, H, D] q"
+    assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, "pools are [pages, page, H_kv, D]"
+    assert k_pages.dtype == v_pages.dtype, "the pools must share a dtype"
+    num_pages, page_size, h_kv, D = k_pages.shape
+    T, H = q.shape[:2]
+    assert q.shape[2] == D and H % h_kv == 0, f"q [{T}, {H}, {q.shape[2]}] does not fit H_kv={h_kv}, D={D}"
+    dev = q.device
+    assert k_pages.device == v_pages.device == dev, "q and the pools must be on one device"
+    nseq = cu_seqlens_q.numel() - 1
+    assert block_table.dim() == 2 and block_table.shape[0] == nseq == seq_lens.numel(), (
+        "block_table, cu_seqlens_q and seq_lens describe different batches")
+    words = 0
+    if tree_mask is not None:
+        assert tree_mask.dim() == 2 and tree_mask.shape[0] == T and tree_mask.dtype == torch.int64, (
+            "tree_mask is int64 [T, words]")
+        assert tree_mask.device == dev, "tree_mask must be on q's device"
+        words = tree_mask.shape[1]
+        tree_mask = tree_mask.contiguous()
+    qd, kd, vd = (norm_descale(d, h_kv, dev) for d in (q_descale, k_descale, v_descale))
+    if softmax_scale is None:
+        softmax_scale = 1.0 / math.sqrt(D)
+    q = rows16(q)
+    ks, vs = pool_strides(k_pages, "k_pages"), pool_strides(v_pages, "v_pages")
+    bt, cu, lens = as_i32(block_table, dev), as_i32(cu_seqlens_q, dev), as_i32(seq_lens, dev)
+    out = torch.empty((T, H, D), dtype=out_dtype_for(q.dtype), device=dev)
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev)
+    lib = _lib.load()
+    with _lib.on_device(dev):
+        ws_bytes = lib.fa4cp_attn_paged_tree_workspace_bytes(H, h_kv, D, max_seqlen_q)
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+        rc = lib.fa4cp_attn_fwd_paged_tree(
+            q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,
+            bt.data_ptr(), page_size, num_pages, bt.shape[1], out.data_ptr(), lse.data_ptr(),
+            cu.data_ptr(), lens.data_ptr(), nseq, int(max_seqlen_q), T, H, h_kv, D,
+            _lib.dtype_code(q.dtype), _lib.dtype_code(k_pages.dtype), _lib.ptr(tree_mask), words,
+            float(softmax_scale), _lib.ptr(qd), _lib.ptr(kd), _lib.ptr(vd), ws.data_ptr(),
+            ws.numel(), _lib.stream_of(q))
+    _lib.check(rc, "attn_fwd_paged_tree")
     _lib.count_launches()
     return out, lse

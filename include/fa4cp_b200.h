@@ -515,6 +515,101 @@ FA4CP_API int fa4cp_convert_f32(const float* src, void* dst, int64_t n, int32_t 
                                 void* stream);
 FA4CP_API int fa4cp_add_f32(float* dst, const float* src, int64_t n, void* stream);
 
+/*
+ * Serving over a PAGED K/V cache: block tables, drafted trees, cache writes.  No counterpart
+ * in the reference, whose K/V is contiguous (its README.md:139-141).
+ *
+ * Pools are [num_pages, page_size, Hkv, D] of f16 | bf16 | e4m3, given by a base pointer and
+ * `*_strides`, a HOST array of the (page, row, head) strides in elements: any layout with a
+ * dense last dimension; pointers and strides 16-byte aligned.  Logical row r of request j is
+ * row r % page_size of page block_table[j * max_pages + r / page_size]; its slot is
+ * page * page_size + r % page_size.  Lengths, slots, tables and node lists are read on the
+ * device and not validated on the host; whatever they hold, no access leaves the tensors.
+ *
+ * fa4cp_paged_block_tables: request j has cached_lens[j] tokens and adds new_lens[j]
+ *   (negative: 0; sums below 2^31).  The pages of its new tokens that table_in (NULL: none
+ *   owned; a row's owned pages come first, the rest is negative) lacks are taken from
+ *   free_pages [num_free] in the order of requests and pages.
+ *   table_in, table_out  int32 [nseq, max_pages], distinct; entries not assigned are copied
+ *   num_free_device      NULL or a device int32: the valid entries of free_pages
+ *   slot_mapping         int64 [num_tokens]: the tokens' slots; -1 without a page and behind
+ *                        the last request
+ *   cu_q, cu_k, seq_lens int32 [nseq+1], [nseq+1], [nseq]: sums of new_lens, sums of and the
+ *                        lengths cached + new
+ *   pages                int32 [2]: pages taken from free_pages; pages that could not be
+ *                        provided (free_pages or the table's rows too short)
+ *
+ * fa4cp_paged_tree_mask: mask int64 [total_q, ceil(max_nodes / 64)], bit m of word w of row
+ *   cu_q[j] + i: node i of tree j sees node 64 w + m (itself and its ancestors).  parents
+ *   int32 [total_q]: the parent's index in its tree, below the child's; anything else: none.
+ *   Rows outside every tree are 0.  max_nodes <= 4096.
+ *
+ * fa4cp_paged_kv_write: rows k, v [num_tokens, Hkv, D] at token strides (elements, 16-byte
+ *   aligned) into the pools at slot_mapping; slots outside [0, num_pages * page_size) are
+ *   skipped.  Same dtype: a copy.  f16 | bf16 into e4m3: satfinite(x / descale[head])
+ *   (descales NULL or float32 [Hkv]).  D x element size a multiple of 16 bytes.
+ *
+ * fa4cp_paged_kv_accept: row cached_lens[j] + i of request j becomes what its row
+ *   cached_lens[j] + accepted[j, i] was, in place, for the leading entries of accepted
+ *   (int32 [nseq, max_accept], max_accept <= 1024) that ascend within
+ *   [0, cu_q[j+1] - cu_q[j]); seq_lens[j] = cached_lens[j] + their number.
+ */
+FA4CP_API int fa4cp_paged_block_tables(const int32_t* cached_lens, const int32_t* new_lens,
+                                       int32_t nseq, const int32_t* free_pages, int32_t num_free,
+                                       const int32_t* num_free_device, int32_t page_size,
+                                       int32_t max_pages, const int32_t* table_in,
+                                       int32_t* table_out, int64_t* slot_mapping,
+                                       int64_t num_tokens, int32_t* cu_q, int32_t* cu_k,
+                                       int32_t* seq_lens, int32_t* pages, void* stream);
+FA4CP_API int fa4cp_paged_tree_mask(const int32_t* parents, const int32_t* cu_q, int32_t nseq,
+                                    int64_t total_q, int32_t max_nodes, int64_t* mask,
+                                    void* stream);
+FA4CP_API int fa4cp_paged_kv_write(const void* k, const void* v, int64_t k_token_stride,
+                                   int64_t v_token_stride, void* k_pages, void* v_pages,
+                                   const int64_t* k_strides, const int64_t* v_strides,
+                                   int64_t num_pages, int32_t page_size,
+                                   const int64_t* slot_mapping, int64_t num_tokens,
+                                   int32_t num_heads_kv, int32_t head_dim, int32_t src_dtype,
+                                   int32_t pool_dtype, const float* k_descale,
+                                   const float* v_descale, void* stream);
+FA4CP_API int fa4cp_paged_kv_accept(void* k_pages, void* v_pages, const int64_t* k_strides,
+                                    const int64_t* v_strides, int32_t num_pages,
+                                    int32_t page_size, const int32_t* block_table,
+                                    int32_t max_pages, const int32_t* cached_lens,
+                                    const int32_t* cu_q, int32_t nseq, const int32_t* accepted,
+                                    int32_t max_accept, int32_t num_heads_kv, int32_t head_dim,
+                                    int32_t dtype, int32_t* seq_lens, void* stream);
+
+/*
+ * Attention of a few new tokens a request over its paged cache: decode (one token) and the
+ * verification of drafted trees.
+ *   q            [total_q, Hq, D] at q_token_stride (elements); f16 | bf16 | e4m3
+ *   K/V pools    as above; q's dtype, or e4m3 under any q
+ *   seq_lens     int32 [nseq]: cached tokens; the request's own n = cu_q[j+1] - cu_q[j] tokens
+ *                are the last of them
+ *   tree_mask    int64 [total_q, mask_words] (fa4cp_paged_tree_mask) or NULL: token i sees
+ *                the new rows 0..i.  Every token sees all rows before the new ones.
+ *   out, lse     [total_q, Hq, D] in q's dtype (bf16 for e4m3), [total_q, Hq] float32 natural
+ *                log; rows that see no key: 0, -inf; rows outside cu_q are left as they are
+ *   page_size    16, 32, 64 or a multiple of 128; a page outside [0, num_pages) reads zeros
+ *   *_descale    NULL or float32 [Hkv], each for an e4m3 operand only
+ *   workspace    fa4cp_attn_paged_tree_workspace_bytes(...) bytes of scratch, 16-byte aligned
+ *                (contents on entry do not matter; calls sharing it must not overlap)
+ * Rows behind seq_lens and rows that a token does not see never reach its result, whatever
+ * they hold.  Supported: head_dim 64, 128, 256.
+ */
+FA4CP_API int64_t fa4cp_attn_paged_tree_workspace_bytes(int32_t num_heads_q, int32_t num_heads_kv,
+                                                        int32_t head_dim, int32_t max_seqlen_q);
+FA4CP_API int fa4cp_attn_fwd_paged_tree(
+    const void* q, int64_t q_token_stride, const void* k_pages, const void* v_pages,
+    const int64_t* k_strides, const int64_t* v_strides, const int32_t* block_table,
+    int32_t page_size, int32_t num_pages, int32_t max_pages, void* out, float* lse,
+    const int32_t* cu_q, const int32_t* seq_lens, int32_t nseq, int32_t max_seqlen_q,
+    int64_t total_q, int32_t num_heads_q, int32_t num_heads_kv, int32_t head_dim, int32_t q_dtype,
+    int32_t kv_dtype, const int64_t* tree_mask, int32_t mask_words, float softmax_scale,
+    const float* q_descale, const float* k_descale, const float* v_descale, void* workspace,
+    int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
