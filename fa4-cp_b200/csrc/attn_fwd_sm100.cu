@@ -1802,7 +1802,9 @@ extern "C" int fa4cp_device_status(int32_t* status, int32_t clear) {
     int z = 0;
     FA4CP_CHECK_CUDA(cudaMemcpyToSymbol(g_attn_status, &z, sizeof(int)));
   }
-  *status = v;
+  int tree = 0;
+  if (int rc = tree_status(&tree, clear != 0)) return rc;
+  *status = v != 0 ? v : tree;
   return FA4CP_OK;
 }
 
