@@ -11,20 +11,35 @@
 //
 // Schedule.  The work is the list of all (request, K/V head, row tile, key tile), in that
 // order; every CTA takes an equal share of consecutive key tiles, whatever the lengths are
-// (they are only known on the device).  A row tile whose keys several CTAs share leaves one
-// partial (O, m, l) each in the workspace, joined by tree_combine_kernel in a fixed order.  A
-// CTA has at most two partials (its first and its last row tile), so the workspace does not
-// depend on the lengths.
+// (they are only known on the device).  A row tile counts kItemCost tiles more than it has, for
+// its Q and its result.  A row tile whose keys several CTAs share leaves one partial (O, m, l)
+// each in the workspace, joined by tree_combine_kernel in a fixed order.  A CTA has at most two
+// partials (its first and its last row tile), so the workspace does not depend on the lengths.
 //
 // CTA roles (one CTA per SM):
-//   warps 0-3  softmax + epilogue, thread t owns row t = TMEM lane t; they load Q, too
-//   warp  4    TMA producer: K_0, V_0, K_1, ... into one ring of tiles, a page piece a lane
-//   warp  5    TMEM allocator + MMA issuer (one thread)
-//   warps 8-15 e4m3 cache only: tiles from the raw ring, widened to f16 into the operand ring
-// TMEM: S0 | S1 (BN fp32 columns each) | O (D columns) | Q (D/2 columns of 16-bit pairs).
-// Q is the A operand of S = Q K^T straight from TMEM: the shared memory that it would take
-// holds K/V tiles in flight instead, and the MMA reads K alone from there.
-// MMA order: S0, S1, PV0, S2, PV1, ...; P overwrites its S buffer as in attn_fwd_kernel.
+//   warps 0-7   two softmax warpgroups, taking key tiles in turn: thread t of either owns row t
+//               = TMEM lane t; each loads half of Q and writes half of the result's columns, too
+//   warp  8     the share's items (row tiles) into a ring that the other roles read; TMA producer
+//               of K, a page piece a lane, and before an item's first K tile its Q rows
+//   warp  10    TMA producer of V (a ring of its own: K runs ahead of V)
+//   warp  9     TMEM allocator + issuer of the S MMAs, warp 11 issuer of the PV MMAs (one
+//               elected lane each: an issuer is held up while the tensor core is busy, so the
+//               waits of one hide behind the other's MMAs)
+//   warps 12-15 e4m3 cache only: V tiles from a raw ring, widened to f16
+// TMEM: 4 S buffers (64 fp32 columns each, 32 at head_dim 256) | O (D columns) | Q (D/2).
+// P(j) lies over S(j), as 16-bit pairs, and is the A operand of O += P V; S(j + buffers) waits
+// for PV(j).  A hand-over between two roles takes 200 to 300 cycles, and a tile has five of
+// them, so it is the number of tiles in flight that counts: four of 64 keys ran 1.5 times as
+// fast as two of 128.  Q is the A operand of S = Q K^T straight from TMEM, so the MMA reads K
+// alone from shared memory; it passes through slots of the K ring, loaded while the item before
+// is still worked on.
+// An e4m3 cache: K is multiplied as it is, by a Q in two e4m3 terms (hi + lo of q x 2^s, which
+// hold a bf16 to 2^-17 of its row's largest value), at twice the rate a term; V is widened to
+// f16, because a P in e4m3 would have to be two terms as well, at three conversions a value.
+// The warpgroups share one running maximum a row, handed from tile to tile through shared
+// memory right after a tile's maximum is known (its exponentials come later), and each keeps
+// its own row sum; so one warpgroup's exponentials overlap the other's waits and maxima.
+// What runs once an item is written as small loops: its instructions come from L2 each time.
 #include <atomic>
 
 #include "common.cuh"
@@ -47,11 +62,26 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: P <= 256
 constexpr int BM = 128;
+// An e4m3 V is attended as f16 values x this factor: 448 x 146 is the largest product that f16
+// holds, 480 x 146 (what NaN's bits would stand for) overflows
+constexpr float kV8Scale = 146.f;
 
 // codes written to the device status word when a bounded wait gives up
 enum : int {
-  kErrEmpty = 0x401, kErrRawEmpty, kErrRawFull, kErrOpEmpty, kErrQFull, kErrKFull, kErrPFull,
-  kErrVFull, kErrOFree, kErrSFull, kErrODone, kErrVFix, kErrDrain
+  kErrEmpty = 0x401, kErrRawFull, kErrVEmpty, kErrQFull, kErrKFull, kErrPFull,
+  kErrVFull, kErrOFree, kErrSFull, kErrSFree, kErrMax, kErrODone, kErrVFix, kErrJoin, kErrMeet, kErrItem,
+  kErrItemFree, kErrQStaged, kErrDrain
+};
+
+constexpr int kItemCost = 6;  // key tiles that a row tile's start and end are worth
+constexpr int kItems = 8;     // ring of items
+
+// A CTA's part of a row tile, as the roles of a CTA pass it on (nt == 0: the share has ended).
+struct Item {
+  int seq, token0, n, len, lim;  // request: first token, tokens, cached rows, those with a page entry
+  int kvh, mtile, kt0, nt, kt;   // K/V head, row tile, first key tile, tiles here, tiles in all
+  uint32_t k_idx;                // K ring index of its Q; its K tiles follow
+  int q_slots;
 };
 
 struct TreeParams {
@@ -72,26 +102,45 @@ struct TreeParams {
   float scale_log2;
 };
 
-template <int D_, int BN_, bool KV8_>
+template <int D_, bool KV8_>
 struct TreeTraits {
-  static constexpr int D = D_, BN = BN_;
+  static constexpr int D = D_, BN = D == 256 ? 32 : 64;  // keys of a tile
   static constexpr bool KV8 = KV8_;
-  static constexpr int NCH = D / 64;                // 128-byte columns of an operand tile
-  static constexpr int TILE_BYTES = BN * D * 2;     // one operand tile (K or V)
-  static constexpr int CHUNK_BYTES = BN * 128;
-  static constexpr int RAW_BYTES = BN * D;          // one e4m3 tile
-  static constexpr int RAW_SLOTS = KV8 ? (D == 64 ? 8 : 6) : 0;
-  static constexpr int SLOTS = KV8 ? (D == 64 ? 6 : 4) : (D == 64 ? 12 : 7);
-  static constexpr int OFF_RAW = SLOTS * TILE_BYTES;
-  static constexpr int OFF_BAR = OFF_RAW + RAW_SLOTS * RAW_BYTES;
-  // op_full, op_empty [SLOTS]; raw_full, raw_empty [RAW_SLOTS]; s_full[2], p_full[2],
-  // o_done[2], q_full, o_free, v_fixed, teardown
-  static constexpr int NUM_BARS = 2 * SLOTS + 2 * RAW_SLOTS + 10;
+  static constexpr int KEL = KV8 ? 1 : 2;             // bytes of a K element
+  static constexpr int K_SWZ = D * KEL >= 128 ? 128 : 64;  // bytes of a swizzled row of K
+  static constexpr int K_COLS = D * KEL / K_SWZ;
+  static constexpr int K_BYTES = BN * D * KEL;
+  static constexpr int V_COLS = D / 64;               // 128-byte columns of a V operand tile
+  static constexpr int V_CHUNK = BN * 128;
+  static constexpr int V_BYTES = BN * D * 2;
+  static constexpr int RAW_BYTES = BN * D;            // one e4m3 V tile
+  static constexpr int KS = KV8 && D == 256 ? 8 : 6, VS = 6, RS = KV8 ? 6 : 0;
+  static_assert(KS * K_BYTES >= BM * D * 2, "the K ring takes the Q of an item whole");
+  static constexpr int OFF_V = KS * K_BYTES;
+  static constexpr int OFF_RAW = OFF_V + VS * V_BYTES;
+  static constexpr int OFF_ROWS = OFF_RAW + RS * RAW_BYTES;
+  // per row: running maximum [BM]; per item parity and warpgroup: maximum, sum, flag [2][2][BM]
+  static constexpr int OFF_ITEMS = OFF_ROWS + BM * 4 + 4 * BM * 12;
+  static constexpr int OFF_BAR = OFF_ITEMS + kItems * 48;
+  // k_full, k_empty [KS]; v_full, v_empty [VS]; r_full, r_empty [RS]; s_full, p_full, o_done
+  // [NB]; max_known[8] (warpgroup, warp), v_fixed[2], q_full, o_free, joined, teardown;
+  // q_staged, item_full, item_free [kItems]
+  static constexpr int NB = 4;  // S buffers
+  static constexpr int NUM_BARS = 2 * (KS + VS + RS) + 3 * NB + 14 + 3 * kItems;
+  // q_staged(i) is waited for before q_staged(i + kItems) can complete: the items between them
+  // take two slots of the K ring each, so the latter needs the former's slots back
+  static_assert(KS < 2 * kItems, "Q staging ring");
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int SMEM_BYTES = OFF_MISC + 128 + 1024;
-  static constexpr int THREADS = KV8 ? 512 : 192;
-  static constexpr int CONV_WARPS = 8;
-  static constexpr int TM_S = 0, TM_O = 2 * BN, TM_Q = TM_O + D;
+  // an e4m3 V tile is widened by one warp (two at head_dim 256), the next tile by the next
+  static constexpr int CONV_WARPS = KV8 ? 4 : 0, CONV_TEAM = D == 256 ? 2 : 1;
+  static constexpr int THREADS = 384 + CONV_WARPS * 32;
+  // setmaxnreg split, in registers a thread of a warpgroup; the launch gives 512 x 128 or
+  // 384 x 168 registers
+  static constexpr int REGS_SOFTMAX = KV8 ? 168 : 184, REGS_CONTROL = KV8 ? 80 : 136, REGS_CONV = 96;
+  static_assert(128 * (2 * REGS_SOFTMAX + REGS_CONTROL) + 32 * CONV_WARPS * REGS_CONV <=
+                    (KV8 ? 512 * 128 : 384 * 168), "register split exceeds the launch allocation");
+  static constexpr int TM_S = 0, TM_O = NB * BN, TM_Q = TM_O + D;
   static_assert(TM_Q + D / 2 <= 512, "TMEM budget");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
@@ -104,6 +153,59 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int 
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
+// mbar_wait with the non-suspending test: the hand-overs between this kernel's roles are short,
+// and waking from a suspended wait costs more than they take.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort, int code, int* status) {
+  if (mbar_test(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_test(bar, parity)) return true;
+    if ((it & 1023u) == 0) {
+      if (*abort) return false;
+      if (*reinterpret_cast<volatile int*>(status) != 0) {  // another CTA already gave up
+        *abort = 1;
+        return false;
+      }
+      if (clock64() - t0 > kWaitLimitCycles) {
+        *abort = 1;
+        atomicCAS(status, 0, code);
+        return false;
+      }
+    }
+  }
+}
+// As make_desc_sw128 with the 64-byte swizzle (mode 4).
+__device__ __forceinline__ uint64_t make_desc_sw64(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  return (make_desc_sw128(saddr, lbo_bytes, sbo_bytes) & ~(7ull << 61)) | (4ull << 61);
+}
+// One lane of a converged warp, chosen by the hardware: code under it stays warp-uniform for the
+// compiler, so descriptors and addresses live in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
 __device__ __forceinline__ void fence_async_shared() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -113,9 +215,9 @@ __device__ __forceinline__ void fence_async_shared() {
 // ---------------------------------------------------------------------------
 // One request as the schedule sees it: its rows and key tiles.  Boundaries outside
 // [0, total_q] and empty requests give no work; an empty cache gives one tile, all masked, so
-// that its rows are written.
+// that its rows are written.  Keys behind the request's table row do not exist.
 struct Request {
-  int token0, n, len, mt, kt;  // first token, tokens, cached rows, row tiles, key tiles
+  int token0, n, len, lim, mt, kt;
 };
 
 template <int BN>
@@ -125,16 +227,25 @@ __device__ __forceinline__ Request load_request(const TreeParams& p, int j) {
   r.token0 = a;
   r.n = (a >= 0 && b > a && b <= p.total_q) ? b - a : 0;
   r.len = max(p.seq_lens[j], 0);
-  r.mt = int((int64_t(r.n) * p.group + BM - 1) / BM);
-  r.kt = max(int((int64_t(r.len) + BN - 1) / BN), 1);
+  r.lim = int(min(int64_t(r.len), int64_t(p.max_pages) * p.page_size));
+  r.mt = (r.n * p.group + BM - 1) / BM;  // total_q * Hq < 2^31
+  r.kt = max(int((int64_t(r.lim) + BN - 1) / BN), 1);
   return r;
 }
 
-// The share of key tiles [t0, t1) of CTA c out of G, and the item that t0 falls into.
+// Tiles are counted with kItemCost more for every row tile: `total` of them, of which CTA c of
+// g takes the c-th equal part.
 struct Share {
-  int64_t t0, t1, total;
+  int64_t t0, t1;        // this CTA's part
+  int64_t total, each;   // each = total / g, the first `rest` CTAs take one more
+  int g, rest;
   int64_t off;  // t0 relative to its request's first tile
   int seq;
+  __device__ __forceinline__ int64_t begin(int c) const { return c * each + min(c, rest); }
+  __device__ __forceinline__ int owner(int64_t x) const {  // the CTA whose part holds tile x
+    const int64_t big = rest * (each + 1);
+    return x < big ? int(x / (each + 1)) : rest + int((x - big) / each);
+  }
 };
 
 // All threads of the CTA.  A thread sums a run of requests, a block scan gives its run's first
@@ -146,9 +257,10 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
   const int per = (p.nseq + int(blockDim.x) - 1) / int(blockDim.x);
   const int j0 = min(tid * per, p.nseq), j1 = min(j0 + per, p.nseq);
   int64_t sum = 0;
+#pragma unroll 1
   for (int j = j0; j < j1; ++j) {
     const Request r = load_request<BN>(p, j);
-    sum += int64_t(p.Hkv) * r.mt * r.kt;
+    sum += int64_t(p.Hkv * r.mt) * (r.kt + kItemCost);
   }
   int64_t inc = sum;
 #pragma unroll
@@ -159,20 +271,24 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
   if (lane == 31) ws[warp] = inc;
   __syncthreads();
   int64_t before = 0, total = 0;
+#pragma unroll 1
   for (int w = 0; w < nw; ++w) {
     if (w < warp) before += ws[w];
     total += ws[w];
   }
   Share s;
   s.total = total;
-  const int64_t g = min(int64_t(G), total);  // no CTA has an empty share between others
-  s.t0 = c < g ? total * c / g : total;
-  s.t1 = c < g ? total * (c + 1) / g : total;
+  s.g = int(min(int64_t(G), total));  // no CTA has an empty share between others
+  s.each = s.g > 0 ? total / s.g : 0;
+  s.rest = int(total - s.each * s.g);
+  s.t0 = c < s.g ? s.begin(c) : total;
+  s.t1 = c < s.g ? s.begin(c + 1) : total;
   int64_t first = before + inc - sum;
   if (s.t0 < s.t1 && first <= s.t0 && s.t0 < first + sum) {
+#pragma unroll 1
     for (int j = j0; j < j1; ++j) {
       const Request r = load_request<BN>(p, j);
-      const int64_t tiles = int64_t(p.Hkv) * r.mt * r.kt;
+      const int64_t tiles = int64_t(p.Hkv * r.mt) * (r.kt + kItemCost);
       if (s.t0 < first + tiles) {
         found[0] = j;
         found[1] = s.t0 - first;
@@ -187,42 +303,48 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
   return s;
 }
 
-// Walks a CTA's share item by item; every role runs its own copy.
+// Walks a CTA's share item by item (warp 8).
 template <int BN>
 struct Walk {
   Request r;
-  int64_t off, left;
-  int seq, kvh, mtile, kt0, nt;  // the current item's K/V head, row tile, first tile, tiles
+  int64_t left;         // counted tiles left of the share, from the current position on
+  int seq, kvh, mtile, at;  // position: `at` counted tiles into the row tile
+  int kt0, nt;          // the key tiles of the current row tile that are this CTA's
   __device__ __forceinline__ void start(const TreeParams& p, const Share& s) {
     seq = s.seq;
-    off = s.off;
     left = s.t1 - s.t0;
     r = load_request<BN>(p, seq);
-    set(p);
+    const int64_t item = s.off / (r.kt + kItemCost);
+    at = int(s.off - item * (r.kt + kItemCost));
+    kvh = int(item) / r.mt;
+    mtile = int(item) - kvh * r.mt;
   }
-  __device__ __forceinline__ void set(const TreeParams&) {
-    const int64_t item = off / r.kt;
-    kt0 = int(off - item * r.kt);
-    kvh = int(item / r.mt);
-    mtile = int(item - int64_t(kvh) * r.mt);
-    nt = int(min(int64_t(r.kt - kt0), left));
-  }
-  // to the next item; false at the end of the share
+  // the next row tile with key tiles for this CTA; false at the end of the share
   __device__ __forceinline__ bool next(const TreeParams& p) {
-    left -= nt;
-    if (left <= 0) return false;
-    off += nt;
-    if (off >= int64_t(p.Hkv) * r.mt * r.kt) {
-      off = 0;
-      do {
+    while (left > 0) {
+      if (r.n > 0) {
+        const int here = int(min(int64_t(r.kt + kItemCost - at), left));
+        kt0 = max(at - kItemCost, 0);
+        nt = max(at + here - kItemCost, 0) - kt0;
+        left -= here;
+        at = 0;
+        if (nt > 0) return true;
+        advance(p);
+      } else {
+        if (seq + 1 >= p.nseq) return false;
         r = load_request<BN>(p, ++seq);
-      } while (r.n == 0 && seq + 1 < p.nseq);
+      }
     }
-    set(p);
-    return true;
+    return false;
   }
-  __device__ __forceinline__ int rows(const TreeParams& p) const {
-    return min(BM, r.n * p.group - mtile * BM);
+  __device__ __forceinline__ void advance(const TreeParams& p) {
+    if (left <= 0) return;
+    if (++mtile < r.mt) return;
+    mtile = 0;
+    if (++kvh < p.Hkv) return;
+    kvh = 0;
+    if (seq + 1 < p.nseq) r = load_request<BN>(p, ++seq);
+    else left = 0;
   }
 };
 
@@ -230,11 +352,11 @@ struct Walk {
 // masks
 // ---------------------------------------------------------------------------
 // 32 visibility bits of row-token `node` (global token `tok`) for keys [key, key + 32).
-__device__ __forceinline__ uint32_t seen32(const TreeParams& p, const Request& r, int64_t tok,
+__device__ __forceinline__ uint32_t seen32(const TreeParams& p, int ctx, int lim, int64_t tok,
                                            int node, int key) {
-  if (key >= r.len) return 0u;
-  uint32_t inside = r.len - key >= 32 ? 0xffffffffu : (1u << (r.len - key)) - 1u;
-  const int d = key - (r.len - r.n);  // the keys' index among the new rows
+  if (key >= lim) return 0u;
+  const uint32_t inside = lim - key >= 32 ? 0xffffffffu : (1u << (lim - key)) - 1u;
+  const int d = key - ctx;  // the keys' index among the new rows
   if (d + 31 < 0) return inside;
   uint32_t bits;
   if (p.mask == nullptr) {
@@ -265,78 +387,42 @@ __device__ __forceinline__ float value16(uint32_t h, bool bf16) {
 // ---------------------------------------------------------------------------
 // the kernel
 // ---------------------------------------------------------------------------
-// One 64-element piece of a query row as 32 registers of 16-bit pairs in the operand type.
-// f16 operands of an e4m3 cache: x * f with f a power of two (exact unless f16 underflows).
-template <bool KV8>
-__device__ __forceinline__ void load_q64(const TreeParams& p, const uint8_t* row, int c, float f,
-                                         uint32_t (&r)[32]) {
-  if (!KV8) {
-    const uint4* src = reinterpret_cast<const uint4*>(row + c * 128);
+// 16 elements of a bf16 query row x f as two e4m3 terms, 4 registers of 4 values each.  With
+// the row's largest magnitude brought to [2^7, 2^8) the first term leaves at most half of its
+// last place, which the second holds exactly (8 significant bits in all) down to 2^-10.
+__device__ __forceinline__ void q16_terms(const uint4 a, const uint4 b, float f, uint32_t (&hi)[4],
+                                          uint32_t (&lo)[4]) {
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint4 x = src[i];
-      r[4 * i] = x.x; r[4 * i + 1] = x.y; r[4 * i + 2] = x.z; r[4 * i + 3] = x.w;
+  for (int k = 0; k < 4; ++k) {
+    float v[4], h[4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      v[2 * e] = __uint_as_float(w[2 * k + e] << 16) * f;
+      v[2 * e + 1] = __uint_as_float(w[2 * k + e] & 0xFFFF0000u) * f;
     }
-  } else if (p.q_dtype == FA4CP_DTYPE_E4M3) {
-    const uint4* src = reinterpret_cast<const uint4*>(row + c * 64);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 x = src[i];
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float a, b, cc, d;
-        unpack_e4m3x4(w[k], a, b, cc, d);
-        r[8 * i + 2 * k] = pack_f16x2(a * f, b * f);
-        r[8 * i + 2 * k + 1] = pack_f16x2(cc * f, d * f);
-      }
-    }
-  } else {
-    const bool bf = p.q_dtype == FA4CP_DTYPE_BF16;
-    const uint4* src = reinterpret_cast<const uint4*>(row + c * 128);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint4 x = src[i];
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        r[4 * i + k] = pack_f16x2(value16(w[k] & 0xFFFFu, bf) * f, value16(w[k] >> 16, bf) * f);
-    }
+    hi[k] = pack_e4m3x4(v[0], v[1], v[2], v[3]);
+    unpack_e4m3x4(hi[k], h[0], h[1], h[2], h[3]);
+    lo[k] = pack_e4m3x4(v[0] - h[0], v[1] - h[1], v[2] - h[2], v[3] - h[3]);
   }
-}
-
-// Largest magnitude of a query row (e4m3 cache: the row is brought to f16 by a power of two).
-template <int D>
-__device__ __forceinline__ float q_absmax(const TreeParams& p, const uint8_t* row) {
-  float m = 0.f;
-  if (p.q_dtype == FA4CP_DTYPE_E4M3) return 448.f;
-  const bool bf = p.q_dtype == FA4CP_DTYPE_BF16;
-  const uint4* src = reinterpret_cast<const uint4*>(row);
-#pragma unroll 8
-  for (int i = 0; i < D / 8; ++i) {
-    const uint4 x = src[i];
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      m = fmaxf(m, fmaxf(fabsf(value16(w[k] & 0xFFFFu, bf)), fabsf(value16(w[k] >> 16, bf))));
-  }
-  return m;
 }
 
 // Rows that see a key whose V row is not finite, after the finite part has been written to
-// dst: the non-finite values themselves are added (their weight is positive).  Rare; reads V
-// again from the pool.
-template <int D, class Store>
-__device__ __noinline__ void add_nonfinite(const TreeParams& p, const Request& r, int seq, int kvh,
-                                           int64_t tok, int node, int key0, int key1, Store dst) {
-  const int ctx = max(r.len - r.n, 0);
-  for (int key = max(key0, ctx); key < min(key1, r.len); ++key) {
-    if (!(seen32(p, r, tok, node, key) & 1u)) continue;
+// their row of the result (16-bit) or of a partial (fp32): the non-finite values themselves are
+// added (their weight is positive), columns [d0, d0 + D / 2).  Rare; reads V again from the pool.
+template <int D>
+__device__ __forceinline__ void add_nonfinite(const TreeParams& p, int seq, int kvh, int ctx, int lim,
+                                              int64_t tok, int node, int key0, int key1, int d0,
+                                              uint16_t* out_row, float* part_row) {
+#pragma unroll 1
+  for (int key = max(max(key0, ctx), 0); key < min(key1, lim); ++key) {
+    if (!(seen32(p, ctx, lim, tok, node, key) & 1u)) continue;
     const int e = key / p.page_size;
-    const int page = e < p.max_pages ? p.block_table[int64_t(seq) * p.max_pages + e] : -1;
+    const int page = p.block_table[int64_t(seq) * p.max_pages + e];
     if (page < 0 || page >= p.num_pages) continue;
     const uint8_t* row = p.v + page * p.v_page + (key - e * p.page_size) * p.v_row + kvh * p.v_head;
-    for (int d = 0; d < D; ++d) {
+#pragma unroll 1
+    for (int d = d0; d < d0 + D / 2; ++d) {
       float x;
       if (p.kv_dtype == FA4CP_DTYPE_E4M3) {
         if ((row[d] & 0x7F) != 0x7F) continue;
@@ -347,542 +433,746 @@ __device__ __noinline__ void add_nonfinite(const TreeParams& p, const Request& r
         if (!nonfinite16(h, bf)) continue;
         x = value16(h, bf);
       }
-      dst.add(d, x);
+      if (part_row != nullptr) {
+        __stcg(part_row + d, __ldcg(part_row + d) + x);
+      } else {
+        const float y = value16(out_row[d], p.out_bf16 != 0) + x;
+        out_row[d] = uint16_t(p.out_bf16 ? pack_bf16x2(y, 0.f) : pack_f16x2(y, 0.f));
+      }
     }
   }
 }
-
-struct AddF32 {
-  float* row;
-  __device__ __forceinline__ void add(int d, float x) const { row[d] += x; }
-};
-struct Add16 {
-  uint16_t* row;
-  int bf16;
-  __device__ __forceinline__ void add(int d, float x) const {
-    const float y = value16(row[d], bf16) + x;
-    row[d] = uint16_t(bf16 ? pack_bf16x2(y, 0.f) : pack_f16x2(y, 0.f));
-  }
-};
 
 template <class TR>
 __global__ void __launch_bounds__(TR::THREADS, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const TreeParams p) {
-  constexpr int D = TR::D, BN = TR::BN, NS = TR::SLOTS, NR = TR::KV8 ? TR::RAW_SLOTS : 1;
+  constexpr int D = TR::D, BN = TR::BN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cta = int(blockIdx.x), G = int(gridDim.x);
-
-  // the schedule's scratch lies where the ring will be (no copy is in flight yet)
-  int64_t* sched = reinterpret_cast<int64_t*>(smem);
-  const Share share = find_share<BN>(p, cta, G, sched, sched + 32);
-  if (share.t0 >= share.t1) {  // uniform for the CTA
-    if (threadIdx.x == 0) p.desc[2 * cta] = make_int4(0, 0, 0, 0);
-    return;
-  }
+  const int cta = int(blockIdx.x);
 
   const uint32_t bar0 = smem_u32(smem + TR::OFF_BAR);
   auto BAR = [&](int i) -> uint32_t { return bar0 + 8u * uint32_t(i); };
-  auto op_full = [&](int s) { return BAR(s); };
-  auto op_empty = [&](int s) { return BAR(NS + s); };
-  auto raw_full = [&](int s) { return BAR(2 * NS + s); };
-  auto raw_empty = [&](int s) { return BAR(2 * NS + TR::RAW_SLOTS + s); };
-  constexpr int B1 = 2 * TR::SLOTS + 2 * TR::RAW_SLOTS;
-  auto s_full = [&](int b) { return BAR(B1 + b); };
-  auto p_full = [&](int b) { return BAR(B1 + 2 + b); };
-  auto o_done = [&](int b) { return BAR(B1 + 4 + b); };
-  const uint32_t q_full = BAR(B1 + 6), o_free = BAR(B1 + 7), v_fixed = BAR(B1 + 8),
-                 td_bar = BAR(B1 + 9);
+  auto k_full = [&](uint32_t i) { return BAR(int(i % TR::KS)); };
+  auto k_empty = [&](uint32_t i) { return BAR(TR::KS + int(i % TR::KS)); };
+  auto v_full = [&](uint32_t i) { return BAR(2 * TR::KS + int(i % TR::VS)); };
+  auto v_empty = [&](uint32_t i) { return BAR(2 * TR::KS + TR::VS + int(i % TR::VS)); };
+  constexpr int BR = 2 * (TR::KS + TR::VS), NR = TR::KV8 ? TR::RS : 1;
+  auto r_full = [&](uint32_t i) { return BAR(BR + int(i % NR)); };
+  auto r_empty = [&](uint32_t i) { return BAR(BR + TR::RS + int(i % NR)); };
+  // parity of tile i's fill of a ring of n slots
+  auto phase = [](uint32_t i, uint32_t n) { return (i / n) & 1u; };
+  constexpr int B1 = BR + 2 * TR::RS, NB = TR::NB, B2 = B1 + 3 * NB;
+  auto s_full = [&](uint32_t i) { return BAR(B1 + int(i % NB)); };
+  auto p_full = [&](uint32_t i) { return BAR(B1 + NB + int(i % NB)); };
+  auto o_done = [&](uint32_t i) { return BAR(B1 + 2 * NB + int(i % NB)); };
+  auto max_known = [&](int wg, int w4) { return BAR(B2 + wg * 4 + w4); };
+  auto v_fixed = [&](int wg) { return BAR(B2 + 8 + wg); };
+  const uint32_t q_full = BAR(B2 + 10), o_free = BAR(B2 + 11), joined = BAR(B2 + 12), td_bar = BAR(B2 + 13);
+  auto q_staged = [&](int i) { return BAR(B2 + 14 + i % kItems); };
+  auto item_full = [&](int i) { return BAR(B2 + 14 + kItems + i % kItems); };
+  auto item_free = [&](int i) { return BAR(B2 + 14 + 2 * kItems + i % kItems); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + TR::OFF_MISC);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile uint32_t* bad = tmem_slot + 4;  // [2][4]: keys of a tile with a non-finite V row
+  volatile uint32_t* bad = tmem_slot + 4;  // [2 warpgroups][2][4]: keys with a non-finite V row
+  volatile float* row_max = reinterpret_cast<volatile float*>(smem + TR::OFF_ROWS);
+  volatile float* end_max = row_max + BM;                // [2 items][2 warpgroups][BM]
+  volatile float* end_sum = end_max + 4 * BM;
+  volatile int* end_bad = reinterpret_cast<volatile int*>(end_sum + 4 * BM);
+  Item* items = reinterpret_cast<Item*>(smem + TR::OFF_ITEMS);
   int* status = &g_tree_status;
 
-  __syncthreads();  // the schedule's scratch has been read
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(op_full(s), TR::KV8 ? TR::CONV_WARPS : 1);
-      mbar_init(op_empty(s), 1);
-    }
-    for (int s = 0; s < TR::RAW_SLOTS; ++s) {
-      mbar_init(raw_full(s), 1);
-      mbar_init(raw_empty(s), TR::CONV_WARPS);
-    }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(s_full(b), 1);
-      mbar_init(p_full(b), 128);
-      mbar_init(o_done(b), 1);
-    }
-    mbar_init(q_full, 128);
-    mbar_init(o_free, 128);
-    mbar_init(v_fixed, 4);
-    mbar_init(td_bar, 1);
-    *abort = 0;
-    p.desc[2 * cta] = make_int4(0, 0, 0, 0);  // this thread names the share's split tile at the end
-    for (int i = 0; i < 8; ++i) bad[i] = 0;
-    fence_mbar_init();
-  }
-  if (warp == 4 && lane == 0) {
+  if (threadIdx.x == 32 * 8) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
+    for (int s = 0; s < TR::KS; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+    }
+    for (int s = 0; s < TR::VS; ++s) {
+      mbar_init(v_full(s), TR::KV8 ? TR::CONV_TEAM : 1);
+      mbar_init(v_empty(s), 1);
+    }
+    for (int s = 0; s < TR::RS; ++s) {
+      mbar_init(r_full(s), 1);
+      mbar_init(r_empty(s), TR::CONV_TEAM);
+    }
+    for (int b = 0; b < NB; ++b) {
+      mbar_init(s_full(b), 1);
+      mbar_init(p_full(b), 4);
+      mbar_init(o_done(b), 1);
+    }
+    mbar_init(v_fixed(0), 4);
+    mbar_init(v_fixed(1), 4);
+    for (int i = 0; i < 8; ++i) mbar_init(max_known(0, i), 1);
+    mbar_init(q_full, 8);
+    mbar_init(o_free, 8);
+    mbar_init(joined, 8);
+    mbar_init(td_bar, 2);
+    for (int i = 0; i < kItems; ++i) {
+      mbar_init(q_staged(i), 32);
+      mbar_init(item_full(i), 1);
+      mbar_init(item_free(i), 11 + TR::CONV_WARPS);  // softmax 8, V, S, PV, converters
+    }
+    *abort = 0;
+    fence_mbar_init();
   }
-  if (warp == 5) {
+  if (threadIdx.x == 0) p.desc[2 * cta] = make_int4(0, 0, 0, 0);  // this thread names a split row tile later
+  if (warp == 9) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
   tc_fence_before();
-  __syncthreads();
+  // (two __syncthreads; the scratch lies where the rings will be, before any copy is in flight)
+  int64_t* sched = reinterpret_cast<int64_t*>(smem);
+  const Share share = find_share<BN>(p, cta, int(gridDim.x), sched, sched + 32);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 8) {
+  // The i-th item, for the other roles' warps; false at the end of the share or on give-up.
+  auto get_item = [&](int i, Item& x) -> bool {
+    const bool ok = mbar_wait(item_full(i), uint32_t(i / kItems) & 1, abort, kErrItem, status);
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    x = items[i % kItems];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(item_free(i));
+    return x.nt > 0;
+  };
+
+  if (share.t0 >= share.t1) {
+    // no work (uniform for the CTA): on to the release of TMEM
+  } else if (warp >= 12) {
     if constexpr (TR::KV8) {
-      // ---------------------------------------------------------- e4m3 -> f16
-      // e4m3 is a subset of f16: each 16-byte piece becomes two pieces of the swizzled operand
-      // tile.  Eight lanes take the 64-byte halves of two rows crosswise (row r from chunk a,
-      // row r + 1 from chunk a ^ 1), so neither the reads nor the writes meet in a bank.
-      setmaxnreg_dec<104>();
-      const int t = threadIdx.x - 256;
-      const int sub = t & 7, half = sub >> 2;
-      const uint32_t tiles = uint32_t(2 * (share.t1 - share.t0));
-      bool ok = true;
-      for (uint32_t i = 0; ok && i < tiles; ++i) {
-        const int rs = int(i % NR), os = int(i % NS);
-        ok = mbar_wait(raw_full(rs), uint32_t(i / NR) & 1, abort, kErrRawFull, status);
-        if (ok && i >= NS)
-          ok = mbar_wait(op_empty(os), (uint32_t(i / NS) & 1) ^ 1, abort, kErrOpEmpty, status);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint8_t* src = smem + TR::OFF_RAW + rs * TR::RAW_BYTES;
-        uint8_t* dst = smem + os * TR::TILE_BYTES;
-        constexpr int PER = BN * D / 16 / 256;  // 16-byte pieces a thread
-        uint4 x[PER];
-        int to[PER];
+      // ---------------------------------------------------------- V: e4m3 -> f16
+      // Bits s eeee mmm moved to f16's places are the value x 2^-8, subnormals included; one
+      // product makes it x kV8Scale, exactly (4 x 7 significant bits), and e4m3's NaN, which
+      // the bits take for 480, infinite.  (The conversion instruction runs at a quarter of the
+      // rate, on the unit that the softmax's exponentials need.)  Each 16-byte piece becomes
+      // two pieces of the swizzled operand tile.  Eight lanes take the 64-byte halves of two
+      // rows crosswise (row r from chunk a, row r + 1 from chunk a ^ 1), so neither the reads
+      // nor the writes meet in a bank.
+      setmaxnreg_dec<TR::REGS_CONV>();
+      constexpr int TEAM = TR::CONV_TEAM, TEAMS = 4 / TEAM;
+      const int team = (warp - 12) / TEAM, t = (warp - 12) % TEAM * 32 + lane;
+      const int half = (t & 7) >> 2, piece = t & 3, unit = t >> 3;
+      const int row0 = unit / TR::V_COLS * 2 + half, a = unit % TR::V_COLS;
+      const int ch = TR::V_COLS > 1 && half ? a ^ 1 : a;
+      const uint8_t* src0 = smem + TR::OFF_RAW + row0 * D + ch * 64 + piece * 16;
+      uint8_t* dst0 = smem + TR::OFF_V + ch * TR::V_CHUNK + row0 * 128;
+      constexpr int PIECES = BN * D / 16 / (32 * TEAM);  // 16-byte pieces a thread
+      constexpr int STEP = 8 * TEAM / TR::V_COLS;        // rows from one to the next
+      const __half2 k146 = __floats2half2_rn(kV8Scale * 256.f, kV8Scale * 256.f);
+      uint32_t i = 0;
+      Item x;
+      for (int item = 0; get_item(item, x); ++item) {
+        bool ok = true;
+        for (int j = 0; j < x.nt; ++j, ++i) {
+          if (int(i % TEAMS) != team) continue;
+          ok = mbar_wait(r_full(i), phase(i, NR), abort, kErrRawFull, status);
+          if (ok && i >= uint32_t(TR::VS))
+            ok = mbar_wait(v_empty(i), phase(i, TR::VS) ^ 1, abort, kErrVEmpty, status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const uint8_t* src = src0 + (i % NR) * TR::RAW_BYTES;
+          uint8_t* dst = dst0 + (i % TR::VS) * TR::V_BYTES;
+#pragma unroll 1
+          for (int u0 = 0; u0 < PIECES; u0 += 4) {
+            uint4 in[4];
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-          const int unit = u * 32 + (t >> 3);
-          const int row = unit / TR::NCH * 2 + half;
-          const int a = unit % TR::NCH;
-          const int ch = TR::NCH > 1 && half ? a ^ 1 : a;
-          const int piece = sub & 3;
-          x[u] = *reinterpret_cast<const uint4*>(src + row * D + ch * 64 + piece * 16);
-          to[u] = ch * TR::CHUNK_BYTES + row * 128 + (((2 * piece) ^ (row & 7)) * 16);
-        }
+            for (int u = 0; u < 4; ++u) in[u] = *reinterpret_cast<const uint4*>(src + (u0 + u) * STEP * D);
 #pragma unroll
-        for (int u = 0; u < PER; ++u) {
-          const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-          uint32_t o[8];
+            for (int u = 0; u < 4; ++u) {
+              const uint32_t w[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
+              uint32_t o[8];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(o[2 * k]) : "h"(uint16_t(w[k] & 0xFFFFu)));
-            asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(o[2 * k + 1]) : "h"(uint16_t(w[k] >> 16)));
+              for (int k = 0; k < 4; ++k) {
+                // bytes b3 b2 b1 b0 -> halfwords (b1, b0) and (b3, b2)
+                const uint32_t lo = __byte_perm(w[k], 0u, 0x1404), hi = __byte_perm(w[k], 0u, 0x3424);
+                o[2 * k] = (lo & 0x80008000u) | ((lo >> 1) & 0x3F803F80u);
+                o[2 * k + 1] = (hi & 0x80008000u) | ((hi >> 1) & 0x3F803F80u);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&o[2 * k + h]), k146);
+                  o[2 * k + h] = *reinterpret_cast<const uint32_t*>(&v);
+                }
+              }
+              const int row = row0 + (u0 + u) * STEP;
+              uint8_t* to = dst + (u0 + u) * STEP * 128;
+              const int at = ((2 * piece) ^ (row & 7)) * 16;
+              *reinterpret_cast<uint4*>(to + at) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(to + (at ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
           }
-          *reinterpret_cast<uint4*>(dst + to[u]) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(dst + (to[u] ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
+          fence_async_shared();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(r_empty(i));
+            mbar_arrive(v_full(i));
+          }
         }
-        fence_async_shared();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(raw_empty(rs));
-          mbar_arrive(op_full(os));
-        }
+        if (!ok) break;
       }
     }
-  } else if (warp >= 4) {
-    if constexpr (TR::KV8) setmaxnreg_dec<88>();
-    if (warp == 4) {
-      // ---------------------------------------------------------- TMA producer
-      // a lane copies one (page piece, 128-byte column) of the tile
-      constexpr int COLS = TR::KV8 ? 1 : TR::NCH;
+  } else if (warp >= 8) {
+    setmaxnreg_dec<TR::REGS_CONTROL>();
+    if (warp == 8 || warp == 10) {
+      // ---------------------------------------------------------- producers
+      // a lane copies one (page piece, swizzled column) of a tile
+      const bool is_v = warp == 10;
+      const int slots = is_v ? (TR::KV8 ? TR::RS : TR::VS) : TR::KS;
+      const int bytes = is_v ? (TR::KV8 ? TR::RAW_BYTES : TR::V_BYTES) : TR::K_BYTES;
+      const int cols = is_v ? (TR::KV8 ? 1 : TR::V_COLS) : TR::K_COLS;
+      const int width = is_v && TR::KV8 ? D : is_v ? 128 : TR::K_SWZ;  // bytes of a column's row
+      const int first_full = is_v ? (TR::KV8 ? BR : 2 * TR::KS) : 0;
+      const CUtensorMap* map = is_v ? &tmV : &tmK;
       const int box = min(p.page_size, BN);
-      const int pieces = BN / box;
-      const int piece = lane / COLS, col = lane - piece * COLS;
-      const bool mine = piece < pieces;
-      constexpr int NSL = TR::KV8 ? NR : NS;
-      constexpr int BYTES = TR::KV8 ? TR::RAW_BYTES : TR::TILE_BYTES;
-      const uint32_t base = smem_u32(smem + (TR::KV8 ? TR::OFF_RAW : 0)) +
-                            uint32_t(TR::KV8 ? piece * box * D
-                                             : col * TR::CHUNK_BYTES + piece * box * 128);
-      const int c0 = col * 64;
-      Walk<BN> w;
-      w.start(p, share);
-      // the page and row of this lane's piece of a tile; -1 (zeros) where the cache has ended
-      auto lookup = [&](int seq, const Request& r, int kt, int& row) -> int {
-        const int64_t key = int64_t(kt) * BN + piece * box;
-        const int64_t e = key / p.page_size;
-        row = int(key - e * p.page_size);
-        if (!mine || key >= r.len || e >= p.max_pages) return -1;
-        const int page = p.block_table[int64_t(seq) * p.max_pages + e];
-        return page >= 0 && page < p.num_pages ? page : -1;
+      const int piece = lane / cols, col = lane - piece * cols;
+      const bool mine = piece < BN / box;
+      const uint32_t base = smem_u32(smem) + uint32_t(is_v ? (TR::KV8 ? TR::OFF_RAW : TR::OFF_V) : 0) +
+                            uint32_t(col * BN * width + piece * box * width);
+      const int c0 = col * width / TR::KEL;
+      uint32_t idx = 0, slot = 0, ph = 0;
+      auto step = [&]() {
+        ++idx;
+        if (++slot == uint32_t(slots)) { slot = 0; ph ^= 1; }
       };
-      int row, page = lookup(w.seq, w.r, w.kt0, row);
-      uint32_t idx = 0;
-      bool ok = true, more = true;
-      while (ok && more) {
-        const int n = w.nt, kt0 = w.kt0, kvh = w.kvh, seq = w.seq;
-        const Request r = w.r;
+      auto wait_slot = [&]() -> bool {
+        const bool got = idx < uint32_t(slots) ||
+                         mbar_wait(BAR(first_full + slots + int(slot)), ph ^ 1, abort, kErrEmpty, status);
+        return __all_sync(0xffffffffu, got);
+      };
+      Walk<BN> w;
+      bool more = true;
+      if (!is_v) {
+        w.start(p, share);
         more = w.next(p);
-        for (int j = 0; ok && j < n; ++j) {
-          // the next tile's page is looked up before this one waits for a slot
-          int nrow = 0, npage = -1;
-          if (j + 1 < n) npage = lookup(seq, r, kt0 + j + 1, nrow);
-          else if (more) npage = lookup(w.seq, w.r, w.kt0, nrow);
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv, ++idx) {
-            const int s = int(idx % NSL);
-            const uint32_t ph = uint32_t(idx / NSL) & 1;
-            const uint32_t full = TR::KV8 ? raw_full(s) : op_full(s);
-            const uint32_t empty = TR::KV8 ? raw_empty(s) : op_empty(s);
-            if (idx >= NSL) ok = mbar_wait(empty, ph ^ 1, abort, kErrEmpty, status);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(full, BYTES);
-            __syncwarp();
-            if (mine)
-              tma_load_4d(base + uint32_t(s * BYTES), kv ? &tmV : &tmK, c0, kvh, row, page, full);
+      }
+      bool ok = true;
+      for (int item = 0; ok; ++item) {
+        Item x;
+        if (is_v) {
+          if (!get_item(item, x)) break;
+        } else {
+          // publish the item
+          if (item >= kItems)
+            ok = mbar_wait(item_free(item), (uint32_t(item / kItems) & 1) ^ 1, abort, kErrItemFree, status);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          x.nt = 0;
+          int rows = 0;
+          constexpr int Q_ROW = D * 2;  // bytes of a bf16 / f16 row (e4m3: half)
+          const int q_row = p.q_dtype == FA4CP_DTYPE_E4M3 ? D : Q_ROW;
+          if (more) {
+            x.seq = w.seq; x.token0 = w.r.token0; x.n = w.r.n; x.len = w.r.len; x.lim = w.r.lim;
+            x.kvh = w.kvh; x.mtile = w.mtile; x.kt0 = w.kt0; x.nt = w.nt; x.kt = w.r.kt;
+            x.k_idx = idx;
+            rows = min(BM, w.r.n * p.group - w.mtile * BM);
+            x.q_slots = (rows * q_row + TR::K_BYTES - 1) / TR::K_BYTES;
           }
+          if (lane == 0) {
+            items[item % kItems] = x;
+            mbar_arrive(item_full(item));
+          }
+          if (!more) break;
+          // its Q rows: 16-byte pieces, swizzled by the row so that a thread a row reads them
+          // without bank conflicts
+          const int per_row = q_row / 16, rows_step = 32 / per_row;  // per_row: 4 .. 32
+          const int per_slot = TR::K_BYTES / q_row;
+          const int c = lane & (per_row - 1);
+          int row = lane / per_row;
+          const int packed = x.mtile * BM + row;
+          int node = packed / p.group, g = packed - node * p.group;
+          for (int s = 0; ok && s < x.q_slots; ++s) {
+            ok = wait_slot();
+            if (!ok) break;
+            const uint32_t dst = smem_u32(smem) + slot * uint32_t(TR::K_BYTES);
+            const int end = min(rows, (s + 1) * per_slot);
+#pragma unroll 1
+            for (; row < end; row += rows_step) {
+              const uint8_t* src = p.q + (int64_t(x.token0) + node) * p.q_stride +
+                                   int64_t(x.kvh * p.group + g) * q_row + c * 16;
+              const uint32_t to = dst + uint32_t((row - s * per_slot) * q_row + ((c ^ (row & 7 & (per_row - 1))) * 16));
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+              g += rows_step;
+              while (g >= p.group) { g -= p.group; ++node; }
+            }
+            if (lane == 0) mbar_arrive(BAR(first_full + int(slot)));  // (Q's arrival is q_staged's)
+            step();
+          }
+          if (!ok) break;
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(q_staged(item)) : "memory");
+        }
+        // the page and row of this lane's piece of tile kt; -1 (zeros) where the cache has ended
+        auto lookup = [&](int kt, int& row) -> int {
+          const int64_t key = int64_t(kt) * BN + piece * box;
+          if (!mine || key >= x.lim) { row = 0; return -1; }
+          const int e = int(key) / p.page_size;
+          row = int(key) - e * p.page_size;
+          return p.block_table[int64_t(x.seq) * p.max_pages + e];
+        };
+        int row, page = lookup(x.kt0, row);
+        for (int j = 0; j < x.nt; ++j) {
+          int nrow = 0, npage = -1;  // asked for before this tile waits for its slot
+          if (j + 1 < x.nt) npage = lookup(x.kt0 + j + 1, nrow);
+          ok = wait_slot();
+          if (!ok) break;
+          const uint32_t full = BAR(first_full + int(slot));
+          if (lane == 0) mbar_arrive_expect_tx(full, uint32_t(bytes));
+          __syncwarp();
+          const bool inside = page >= 0 && page < p.num_pages;
+          if (mine) tma_load_4d(base + slot * uint32_t(bytes), map, c0, x.kvh, row, inside ? page : -1, full);
+          step();
           row = nrow;
           page = npage;
+        }
+        if (!is_v && ok) {
+          w.advance(p);
+          more = w.next(p);
         }
       }
       // every copy that was issued has landed before the CTA ends (on the normal path the
       // consumers have waited for them)
-      for (uint32_t i = idx > NSL ? idx - NSL : 0; i < idx; ++i) {
-        const int s = int(i % NSL);
-        mbar_wait_drain(TR::KV8 ? raw_full(s) : op_full(s), uint32_t(i / NSL) & 1, kErrDrain, status);
-      }
-    } else if (warp == 5 && lane == 0) {
-      // ---------------------------------------------------------- MMA issuer
-      const int fmt = p.kv_dtype == FA4CP_DTYPE_BF16 ? 1 : 0;  // an e4m3 cache is attended in f16
-      const uint32_t idesc_qk = make_idesc(BM, BN, fmt, fmt, 0, 0);
-      const uint32_t idesc_pv = make_idesc(BM, D, fmt, fmt, 0, 1);
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      for (uint32_t i = idx > uint32_t(slots) ? idx - slots : 0; i < idx; ++i)
+        mbar_wait_drain(BAR(first_full + int(i % slots)), (i / slots) & 1, kErrDrain, status);
+    } else {
+      // ---------------------------------------------------------- MMA issuers
+      // A warp walks the tiles together and one elected lane issues: descriptors then stay in
+      // uniform registers (issuing from one lane's own branch took 1.3 times as long).
+      const int fmt = p.kv_dtype == FA4CP_DTYPE_BF16 ? 1 : 0;  // (e4m3 is format 0, and V is f16)
       const uint32_t ring = smem_u32(smem);
-      Walk<BN> w;
-      w.start(p, share);
       uint32_t it = 0;
-      int item = 0;
-      bool ok = true, more = true;
-      auto issue_pv = [&](uint32_t i, bool first) -> bool {
-        const int b = int(i & 1), s = int((2 * i + 1) % NS);
-        if (!mbar_wait(p_full(b), uint32_t(i >> 1) & 1, abort, kErrPFull, status)) return false;
-        if (!mbar_wait(op_full(s), uint32_t((2 * i + 1) / NS) & 1, abort, kErrVFull, status)) return false;
-        if (first && item > 0 && !mbar_wait(o_free, uint32_t(item - 1) & 1, abort, kErrOFree, status))
-          return false;
-        tc_fence_after();
-        const uint32_t sV = ring + uint32_t(s * TR::TILE_BYTES);
+      Item x;
+      if (warp == 9) {
+        const uint32_t idesc = make_idesc(BM, BN, fmt, fmt, 0, 0);
+        const int q_terms = TR::KV8 && p.q_dtype != FA4CP_DTYPE_E4M3 ? 2 : 1;
+        // 32 bytes along D a step, then the next swizzled column
+        constexpr int STEPS = D * TR::KEL / 32, PER_COL = TR::K_SWZ / 32;
+        for (int item = 0; get_item(item, x); ++item) {
+          bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, uint32_t(item) & 1, abort, kErrQFull, status));
+          if (!ok) break;
+          if (lane < x.q_slots) mbar_arrive(k_empty(x.k_idx + lane));  // Q has been read
+          uint32_t ki = x.k_idx + x.q_slots;
+          for (int j = 0; j < x.nt; ++j, ++it, ++ki) {
+            if (it >= uint32_t(NB))  // the P over the buffer's last S has been multiplied
+              ok = mbar_wait(o_done(it - NB), phase(it - NB, NB), abort, kErrSFree, status);
+            if (ok) ok = mbar_wait(k_full(ki), phase(ki, TR::KS), abort, kErrKFull, status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t sK = ring + (ki % TR::KS) * TR::K_BYTES;
+            const uint64_t desc = TR::K_SWZ == 128 ? make_desc_sw128(sK, 16, 1024) : make_desc_sw64(sK, 16, 512);
+            const uint32_t d = tmem + uint32_t(TR::TM_S) + it % NB * BN, a = tmem + uint32_t(TR::TM_Q);
+            if (elect_one()) {
+              if constexpr (TR::KV8) {
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
-          const uint64_t bdesc = make_desc_sw128(sV + kk * 16 * 128, TR::CHUNK_BYTES, 1024);
-          mma_f16_ts(tmem + TR::TM_O, tmem + uint32_t(TR::TM_S + b * BN + kk * 8), bdesc, idesc_pv,
-                     (!first || kk > 0) ? 1u : 0u);
-        }
-        tc_commit(o_done(b));
-        tc_commit(op_empty(s));
-        return true;
-      };
-      while (ok && more) {
-        const int n = w.nt;
-        more = w.next(p);
-        ok = mbar_wait(q_full, uint32_t(item) & 1, abort, kErrQFull, status);
-        tc_fence_after();
-        for (int j = 0; ok && j < n; ++j, ++it) {
-          const int b = int(it & 1), s = int((2 * it) % NS);
-          if (!mbar_wait(op_full(s), uint32_t((2 * it) / NS) & 1, abort, kErrKFull, status)) { ok = false; break; }
-          tc_fence_after();
-          const uint32_t sK = ring + uint32_t(s * TR::TILE_BYTES);
+                for (int kk = 0; kk < STEPS; ++kk)
+                  mma_f8_ts(d, a + uint32_t(kk * 8), desc + uint64_t((kk / PER_COL * BN * TR::K_SWZ + kk % PER_COL * 32) / 16),
+                            idesc, kk > 0 ? 1u : 0u);
+                if (q_terms == 2) {
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const int off = kk * 32;  // bytes along D
-            const uint64_t bdesc =
-                make_desc_sw128(sK + (off / 128) * TR::CHUNK_BYTES + (off % 128), 16, 1024);
-            mma_f16_ts(tmem + uint32_t(TR::TM_S + b * BN), tmem + uint32_t(TR::TM_Q + kk * 8), bdesc,
-                       idesc_qk, kk > 0 ? 1u : 0u);
+                  for (int kk = 0; kk < STEPS; ++kk)
+                    mma_f8_ts(d, a + uint32_t(D / 4 + kk * 8),
+                              desc + uint64_t((kk / PER_COL * BN * TR::K_SWZ + kk % PER_COL * 32) / 16), idesc, 1u);
+                }
+              } else {
+#pragma unroll
+                for (int kk = 0; kk < STEPS; ++kk)
+                  mma_f16_ts(d, a + uint32_t(kk * 8), desc + uint64_t((kk / PER_COL * BN * TR::K_SWZ + kk % PER_COL * 32) / 16),
+                             idesc, kk > 0 ? 1u : 0u);
+              }
+              tc_commit(s_full(it));
+              tc_commit(k_empty(ki));
+            }
+            __syncwarp();
           }
-          tc_commit(s_full(b));
-          tc_commit(op_empty(s));
-          if (j > 0 && !issue_pv(it - 1, j == 1)) ok = false;
+          if (!ok) break;
         }
-        if (ok) ok = issue_pv(it - 1, n == 1);
-        ++item;
+      } else {
+        const uint32_t idesc = make_idesc(BM, D, fmt, fmt, 0, 1);
+        for (int item = 0; get_item(item, x); ++item) {
+          bool ok = true;
+          for (int j = 0; j < x.nt; ++j, ++it) {
+            if (j == 0 && item > 0) ok = mbar_wait(o_free, uint32_t(item - 1) & 1, abort, kErrOFree, status);
+            if (ok) ok = mbar_wait(v_full(it), phase(it, TR::VS), abort, kErrVFull, status);
+            if (ok) ok = mbar_wait(p_full(it), phase(it, NB), abort, kErrPFull, status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t desc = make_desc_sw128(ring + TR::OFF_V + (it % TR::VS) * TR::V_BYTES, TR::V_CHUNK, 1024);
+            if (elect_one()) {
+#pragma unroll
+              for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys: 16 rows of 128 bytes further
+                mma_f16_ts(tmem + TR::TM_O, tmem + uint32_t(TR::TM_S + kk * 8) + it % NB * BN, desc + uint64_t(kk * 16 * 128 / 16),
+                           idesc, (j > 0 || kk > 0) ? 1u : 0u);
+              tc_commit(o_done(it));
+              tc_commit(v_empty(it));
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+        }
       }
       // every MMA issued above has completed before TMEM is released
-      tc_commit(td_bar);
+      if (elect_one()) tc_commit(td_bar);
+      __syncwarp();
       mbar_wait_drain(td_bar, 0, kErrDrain, status);
     }
   } else {
     // ------------------------------------------------------------ softmax + epilogue
-    if constexpr (TR::KV8) setmaxnreg_inc<216>();
-    const int t = threadIdx.x;  // 0..127
-    const uint32_t t_lane = tmem + (uint32_t(warp * 32) << 16);
+    setmaxnreg_inc<TR::REGS_SOFTMAX>();
+    const int wg = warp >> 2, w4 = warp & 3;
+    const int t = threadIdx.x & 127;  // row of the tile
+    const uint32_t t_lane = tmem + (uint32_t(w4 * 32) << 16);
     const bool bf16_op = p.kv_dtype == FA4CP_DTYPE_BF16;
-    Walk<BN> w;
-    w.start(p, share);
-    float qf = 1.f;  // the row's power of two (e4m3 cache)
+    const bool q8 = p.q_dtype == FA4CP_DTYPE_E4M3;
+    // One arrival a warp, for its lanes' TMEM (and shared memory) accesses so far.
+    auto warp_arrive = [&](uint32_t bar) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
+    float qf = 1.f;  // the row's factor (e4m3 cache): a power of two, with the descales' sign
 
-    // Q of item `w` into TMEM.  All S MMAs of the item before are complete (this thread has
-    // seen its last s_full).
-    auto load_q = [&](const Walk<BN>& x) {
-      const int r = x.mtile * BM + t;
-      const bool valid = t < x.rows(p);
-      if (warp * 32 < x.rows(p)) {  // the warp has rows; the others' lanes are never read
-        const int node = r / p.group, head = x.kvh * p.group + (r - node * p.group);
-        const uint8_t* row = p.q + (int64_t(x.r.token0) + (valid ? node : 0)) * p.q_stride +
-                             int64_t(valid ? head : 0) * D * (p.q_dtype == FA4CP_DTYPE_E4M3 ? 1 : 2);
-        if (TR::KV8) {
-          // largest magnitude into [2^14, 2^15): f16 then holds the row to 2^-24 of it
-          const uint32_t e = __float_as_uint(q_absmax<D>(p, row)) >> 23;
-          const int s = e == 0 || e == 255 ? 0 : min(127 + 14 - int(e), 126);
-          qf = __uint_as_float(uint32_t(127 + s) << 23);
-          if ((p.q_descale ? p.q_descale[x.kvh] : 1.f) * (p.k_descale ? p.k_descale[x.kvh] : 1.f) < 0.f) qf = -qf;
+    // This warpgroup's half of item `x`'s Q into TMEM.  All S MMAs of the item before are
+    // complete (the caller has seen its last s_full).
+    auto load_q = [&](const Item& x, int item) -> bool {
+      const bool ok = mbar_wait(q_staged(item), uint32_t(item / kItems) & 1, abort, kErrQStaged, status);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      const int rows = min(BM, x.n * p.group - x.mtile * BM);
+      if (w4 * 32 < rows) {  // the warp has rows; the others' lanes are never read
+        const int row = min(t, rows - 1);
+        const int q_row = q8 ? D : 2 * D, per_slot = TR::K_BYTES / q_row;
+        const int s = row / per_slot, swz = row & 7 & (q_row / 16 - 1);
+        const uint8_t* src = smem + (x.k_idx + s) % TR::KS * TR::K_BYTES + (row - s * per_slot) * q_row;
+        auto piece = [&](int c) { return *reinterpret_cast<const uint4*>(src + ((c ^ swz) * 16)); };
+        float mul = 1.f;
+        if constexpr (TR::KV8) {
+          int e = 0;
+          bool finite = true;
+          if (!q8) {
+            uint32_t top = 0;  // largest magnitude, as bits of a bf16
+#pragma unroll 4
+            for (int c = 0; c < D / 8; ++c) {
+              const uint4 v = piece(c);
+              top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu),
+                                           __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+            }
+            const int exp = int(max(top & 0xFFFFu, top >> 16)) >> 7;
+            finite = exp != 255;
+            if (exp != 0 && finite) e = min(127 + 7 - exp, 126);
+          }
+          qf = __uint_as_float(uint32_t(127 + e) << 23);
+          // a row with infinities or NaN is NaN all over
+          mul = finite ? qf : __uint_as_float(0x7FC00000u);
+          if ((p.q_descale ? p.q_descale[x.kvh] : 1.f) * (p.k_descale ? p.k_descale[x.kvh] : 1.f) < 0.f) {
+            qf = -qf;
+            mul = -mul;
+          }
         }
 #pragma unroll 1
-        for (int c = 0; c < D / 64; ++c) {
-          uint32_t reg[32];
-          load_q64<TR::KV8>(p, row, c, qf, reg);
-          tmem_st32(t_lane + uint32_t(TR::TM_Q + c * 32), reg);
+        for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c) {  // 32 elements
+          if constexpr (TR::KV8) {
+            uint32_t hi[8], lo[8];
+            if (q8) {
+              const uint32_t flip = mul < 0.f ? 0x80808080u : 0u;
+              const uint4 a = piece(2 * c), b = piece(2 * c + 1);
+              hi[0] = a.x ^ flip; hi[1] = a.y ^ flip; hi[2] = a.z ^ flip; hi[3] = a.w ^ flip;
+              hi[4] = b.x ^ flip; hi[5] = b.y ^ flip; hi[6] = b.z ^ flip; hi[7] = b.w ^ flip;
+            } else {
+              uint32_t h[4], o[4];
+              q16_terms(piece(4 * c), piece(4 * c + 1), mul, h, o);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) { hi[k] = h[k]; lo[k] = o[k]; }
+              q16_terms(piece(4 * c + 2), piece(4 * c + 3), mul, h, o);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) { hi[4 + k] = h[k]; lo[4 + k] = o[k]; }
+              tmem_st8(t_lane + uint32_t(TR::TM_Q + D / 4 + c * 8), lo);
+            }
+            tmem_st8(t_lane + uint32_t(TR::TM_Q + c * 8), hi);
+          } else {
+            uint32_t r[16];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint4 v = piece(4 * c + k);
+              r[4 * k] = v.x; r[4 * k + 1] = v.y; r[4 * k + 2] = v.z; r[4 * k + 3] = v.w;
+            }
+            tmem_st16(t_lane + uint32_t(TR::TM_Q + c * 16), r);
+          }
         }
         tmem_wait_st();
       }
-      tc_fence_before();
-      mbar_arrive(q_full);
+      warp_arrive(q_full);
+      return true;
     };
 
-    load_q(w);
-    uint32_t it = 0, fixes = 0;
-    bool aborted = false, more = true;
-    while (more && !aborted) {
-      const Request r = w.r;
-      const int seq = w.seq, kvh = w.kvh, kt0 = w.kt0, n = w.nt, mtile = w.mtile;
-      const int rows = w.rows(p);
-      const bool active = warp * 32 < rows;
-      const int packed = mtile * BM + t;
+    Item x;
+    uint32_t it0 = 0, fixes = 0;  // the item's first tile, counted over the share
+    int item = 0;
+    bool ok = true;
+    bool more = get_item(0, x), aborted = false;
+    if (more) more = load_q(x, 0);
+    while (more) {
+      const int n = x.nt;
+      const int rows = min(BM, x.n * p.group - x.mtile * BM);
+      const bool active = w4 * 32 < rows;
       const bool valid = t < rows;
-      const int node = valid ? packed / p.group : 0;
-      const int head = kvh * p.group + (valid ? packed - node * p.group : 0);
-      const int64_t tok = int64_t(r.token0) + node;
-      const int ctx = r.len - r.n;
+      const int packed = x.mtile * BM + (valid ? t : 0);
+      const int node = packed / p.group;
+      const int head = x.kvh * p.group + (packed - node * p.group);
+      const int64_t tok = int64_t(x.token0) + node;
+      const int ctx = x.len - x.n;
       float scale = p.scale_log2, vscale = 1.0f;
       if (TR::KV8) {
-        if (p.q_descale) scale *= p.q_descale[kvh];
-        if (p.k_descale) scale *= p.k_descale[kvh];
-        if (p.v_descale) vscale = p.v_descale[kvh];
+        if (p.q_descale) scale *= p.q_descale[x.kvh];
+        if (p.k_descale) scale *= p.k_descale[x.kvh];
+        if (p.v_descale) vscale = p.v_descale[x.kvh];
+        vscale *= 1.f / kV8Scale;
         // qf carries the sign of the descales, so the scale is positive; never 0, so that a
         // masked score stays -inf
         scale /= qf;
         scale = scale < 1.17549435e-38f ? 1.17549435e-38f : scale;
       }
+      // m: the maximum that O and this warpgroup's sum l are relative to, as far as this
+      // warpgroup knows
       float m = kNegInf, l = 0.f;
       bool sees_bad = false;
-
-      for (int j = 0; j < n; ++j, ++it) {
-        const int b = int(it & 1);
-        bool ok = mbar_wait(s_full(b), uint32_t(it >> 1) & 1, abort, kErrSFull, status);
+      for (int j = (it0 & 1) == uint32_t(wg) ? 0 : 1; j < n; j += 2) {
+        const uint32_t it = it0 + j;
+        ok = mbar_wait(s_full(it), phase(it, NB), abort, kErrSFull, status);
         if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
         tc_fence_after();
-        const int kbase = (kt0 + j) * BN;
-        const bool edge = kbase + BN > ctx;  // the tile holds new rows, or the cache's end
-        uint32_t vis[BN / 32];
-        if (active) {
-          uint32_t sr[BN / 32][32];
+        const int kbase = (x.kt0 + j) * BN;
+        const bool edge = kbase + BN > ctx || kbase + BN > x.lim;  // new rows, or the cache's end
+        const uint32_t t_s = t_lane + uint32_t(TR::TM_S) + it % NB * BN;
+        constexpr int C = BN / 32;
+        uint32_t vis[C];
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) tmem_ld32(t_lane + uint32_t(TR::TM_S + b * BN + c * 32), sr[c]);
+        for (int c = 0; c < C; ++c) vis[c] = 0u;
+        // the tile before has settled the maximum (the other warpgroup's tile)
+        auto max_settled = [&]() -> bool {
+          return it == 0 || __all_sync(0xffffffffu, mbar_wait(max_known(wg ^ 1, w4), ((it - 1) >> 1) & 1, abort,
+                                                              kErrMax, status));
+        };
+        if (active) {
+          uint32_t sr[C][32];
+#pragma unroll
+          for (int c = 0; c < C; ++c) tmem_ld32(t_s + uint32_t(c * 32), sr[c]);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c) reg_fence32(sr[c]);
+          for (int c = 0; c < C; ++c) reg_fence32(sr[c]);
           if (edge) {
 #pragma unroll
-            for (int c = 0; c < BN / 32; ++c) {
-              vis[c] = seen32(p, r, tok, node, kbase + c * 32);
+            for (int c = 0; c < C; ++c) {
+              vis[c] = seen32(p, ctx, x.lim, tok, node, kbase + c * 32);
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (!((vis[c] >> e) & 1u)) sr[c][e] = __float_as_uint(kNegInf);
             }
           }
-          float mx[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+          float mx4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
-          for (int c = 0; c < BN / 32; ++c)
+          for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int e = 0; e < 32; e += 8)
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                mx[k] = fmax3(mx[k], __uint_as_float(sr[c][e + 2 * k]), __uint_as_float(sr[c][e + 2 * k + 1]));
-          const float m_new = fmaxf(fmax3(m, mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-          if (j == 0) {
+                mx4[k] = fmax3(mx4[k], __uint_as_float(sr[c][e + 2 * k]), __uint_as_float(sr[c][e + 2 * k + 1]));
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+          if (!max_settled()) { aborted = true; break; }
+          float so_far = kNegInf;
+          if (j > 0) so_far = row_max[t];
+          // raised only when it would grow by more than 2^8, or comes to exist
+          const bool need = j > 0 && (so_far == kNegInf ? mx != kNegInf : (mx - so_far) * scale > kRescaleThreshold);
+          const float m_new = need || j == 0 ? mx : so_far;
+          row_max[t] = m_new;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(max_known(wg, w4));
+          // from here on off the other warpgroup's way
+          if (m_new != m) {
+            if (m != kNegInf) l *= ex2_approx((m - m_new) * scale);
             m = m_new;
-          } else {
-            const bool need = (m_new - m) * scale > kRescaleThreshold;
-            if (__any_sync(0xffffffffu, need)) {
-              const float f = need ? ex2_approx((m - m_new) * scale) : 1.0f;
-              if (need) { l *= f; m = m_new; }
-              ok = mbar_wait(o_done(b ^ 1), uint32_t((it - 1) >> 1) & 1, abort, kErrODone, status);
-              if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
-              tc_fence_after();
+          }
+          if (__any_sync(0xffffffffu, need)) {
+            const float f = !need ? 1.f : so_far == kNegInf ? 0.f : ex2_approx((so_far - m_new) * scale);
+            ok = mbar_wait(o_done(it - 1), phase(it - 1, NB), abort, kErrODone, status);
+            if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
+            tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld32(t_lane + uint32_t(TR::TM_O + c * 32), o);
-                tmem_wait_ld();
-                reg_fence32(o);
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16(t_lane + uint32_t(TR::TM_O + c * 16), o);
+              tmem_wait_ld();
+              reg_fence16(o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st32(t_lane + uint32_t(TR::TM_O + c * 32), o);
-              }
-              tmem_wait_st();
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(t_lane + uint32_t(TR::TM_O + c * 16), o);
             }
           }
           const float neg_m = (m == kNegInf) ? 0.f : -m * scale;
           const uint64_t scale2 = f2pack(scale, scale), negm2 = f2pack(neg_m, neg_m);
           uint64_t rs[2] = {0ull, 0ull};
+          uint32_t pw[C][16];
 #pragma unroll
-          for (int hf = 0; hf < BN / 64; ++hf) {
-            uint32_t pw[32];
+          for (int c = 0; c < C; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int c = hf * 2 + (i >> 4), e = (2 * i) & 31;
-              const uint64_t x = ffma2(f2pack(__uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1])), scale2, negm2);
-              const float x0 = ex2_approx(f2lo(x)), x1 = ex2_approx(f2hi(x));
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t y = ffma2(f2pack(__uint_as_float(sr[c][2 * i]), __uint_as_float(sr[c][2 * i + 1])), scale2, negm2);
+              const float x0 = ex2_approx(f2lo(y)), x1 = ex2_approx(f2hi(y));
               rs[i & 1] = fadd2(rs[i & 1], f2pack(x0, x1));
-              pw[i] = !TR::KV8 && bf16_op ? pack_bf16x2(x0, x1) : pack_f16x2(x0, x1);
+              pw[c][i] = !TR::KV8 && bf16_op ? pack_bf16x2(x0, x1) : pack_f16x2(x0, x1);
             }
-            tmem_st32(t_lane + uint32_t(TR::TM_S + b * BN + hf * 32), pw);
-          }
+#pragma unroll
+          for (int c = 0; c < C; ++c) tmem_st16(t_s + uint32_t(c * 16), pw[c]);
           const uint64_t rsum = fadd2(rs[0], rs[1]);
           l += f2lo(rsum) + f2hi(rsum);
+        } else {
+          if (!max_settled()) { aborted = true; break; }
+          if (lane == 0) mbar_arrive(max_known(wg, w4));
         }
         if (edge) {
           // P is 0 where a row does not look, but 0 * NaN is NaN: V rows behind the cache are
           // cleared, and so are the non-finite values of new rows (a context row is seen by
-          // every token, so its values go through as they are).  Thread t has key t.
-          const int s = int((2 * it + 1) % NS);
-          ok = mbar_wait(op_full(s), uint32_t((2 * it + 1) / NS) & 1, abort, kErrVFix, status);
+          // every token, so its values go through as they are).  Thread t has key t % BN, and its
+          // share of the columns.
+          ok = mbar_wait(v_full(it), phase(it, TR::VS), abort, kErrVFix, status);
           if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
-          const int key = kbase + t;
-          uint8_t* vrow = smem + s * TR::TILE_BYTES + t * 128;
+          constexpr int PER = D / 8 * BN / 128;  // 16-byte pieces of a thread
+          const int key = kbase + (t & (BN - 1));
+          uint8_t* vrow = smem + TR::OFF_V + (it % TR::VS) * TR::V_BYTES + (t & (BN - 1)) * 128;
           bool mine_bad = false;
-          if (t < BN && key >= r.len) {
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c)
-              *reinterpret_cast<uint4*>(vrow + (c >> 3) * TR::CHUNK_BYTES + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
-          } else if (t < BN && key >= ctx && r.n > 1) {
-#pragma unroll 4
-            for (int c = 0; c < D / 8; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(vrow + (c >> 3) * TR::CHUNK_BYTES + (c & 7) * 16);
-              uint32_t x[4] = {at->x, at->y, at->z, at->w};
-              bool hit = false;
+          if (key >= x.lim || (key >= ctx && x.n > 1)) {
+#pragma unroll 1
+            for (int c = t / BN * PER; c < (t / BN + 1) * PER; ++c) {
+              uint4* at = reinterpret_cast<uint4*>(vrow + (c >> 3) * TR::V_CHUNK + (c & 7) * 16);
+              const uint4 v = *at;
+              uint32_t y[4] = {v.x, v.y, v.z, v.w};
+              bool hit = key >= x.lim;
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                if (nonfinite16(x[k] & 0xFFFFu, bf16_op)) { x[k] &= 0xFFFF0000u; hit = true; }
-                if (nonfinite16(x[k] >> 16, bf16_op)) { x[k] &= 0xFFFFu; hit = true; }
+                if (key >= x.lim) y[k] = 0;
+                if (nonfinite16(y[k] & 0xFFFFu, bf16_op)) { y[k] &= 0xFFFF0000u; hit = mine_bad = true; }
+                if (nonfinite16(y[k] >> 16, bf16_op)) { y[k] &= 0xFFFFu; hit = mine_bad = true; }
               }
-              if (hit) {
-                *at = make_uint4(x[0], x[1], x[2], x[3]);
-                mine_bad = true;
-              }
+              if (hit) *at = make_uint4(y[0], y[1], y[2], y[3]);
             }
           }
           fence_async_shared();
-          if (r.n > 1) {
+          if (x.n > 1) {
             // which keys of the tile were cleared: one word a warp, two sets used in turn
             const uint32_t word = __ballot_sync(0xffffffffu, mine_bad);
-            volatile uint32_t* set = bad + (fixes & 1) * 4;
+            volatile uint32_t* set = bad + wg * 8 + (fixes & 1) * 4;
             if (lane == 0) {
-              set[warp] = word;
-              mbar_arrive(v_fixed);
+              set[w4] = word;
+              mbar_arrive(v_fixed(wg));
             }
-            ok = mbar_wait(v_fixed, fixes & 1, abort, kErrVFix, status);
+            ok = mbar_wait(v_fixed(wg), fixes & 1, abort, kErrVFix, status);
             if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
             ++fixes;
-            if (active) {
 #pragma unroll
-              for (int c = 0; c < BN / 32; ++c) sees_bad |= (set[c] & vis[c]) != 0;
-            }
+            for (int i = 0; i < 4; ++i) sees_bad |= active && (set[i] & vis[i % C]) != 0;
           }
         }
         if (active) tmem_wait_st();
-        tc_fence_before();
-        mbar_arrive(p_full(b));
+        warp_arrive(p_full(it));
       }
       if (aborted) break;
 
-      // the next item's Q goes in before this item's epilogue, so its first S starts meanwhile
-      const int64_t left_after = w.left - w.nt;
-      const bool whole = kt0 == 0 && n == r.kt;
-      const bool begins = kt0 == 0;
-      more = w.next(p);
-      if (more) load_q(w);
+      // what the other warpgroup needs to finish the row
+      const uint32_t last = it0 + n - 1;
+      const int set = (item & 1) * 2;
+      end_max[(set + wg) * BM + t] = m;
+      end_sum[(set + wg) * BM + t] = l;
+      end_bad[(set + wg) * BM + t] = sees_bad;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(joined);
 
-      const uint32_t last = it - 1;
-      bool ok = mbar_wait(o_done(int(last & 1)), uint32_t(last >> 1) & 1, abort, kErrODone, status);
-      if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
+      // the next item's Q goes in before this item's epilogue, so its first S starts meanwhile
+      ok = mbar_wait(s_full(last), phase(last, NB), abort, kErrSFull, status);
+      if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      const int part = 2 * cta + (begins ? 1 : 0);
-      const float ms = m == kNegInf ? kNegInf : m * scale;  // log2 units
+      Item y;
+      more = get_item(item + 1, y);
+      if (more && !load_q(y, item + 1)) break;
+
+      ok = mbar_wait(joined, uint32_t(item) & 1, abort, kErrJoin, status);
+      if (ok) ok = mbar_wait(o_done(last), phase(last, NB), abort, kErrODone, status);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      // the last tile's warpgroup knows the maximum that O is relative to
+      m = end_max[(set + int(last & 1)) * BM + t];
+      l = 0.f;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        const float mg = end_max[(set + g) * BM + t], lg = end_sum[(set + g) * BM + t];
+        l += mg == m || mg == kNegInf ? lg : lg * ex2_approx((mg - m) * scale);
+        sees_bad |= end_bad[(set + g) * BM + t] != 0;
+      }
+      const bool whole = n == x.kt;
+      const int part = 2 * cta + (x.kt0 == 0 ? 1 : 0);
       const float mult = whole ? (l == 0.f ? 0.f : vscale / l) : vscale;
-      const int64_t orow = (tok * p.Hq + head) * D;
+      uint16_t* out_row = static_cast<uint16_t*>(p.out) + (tok * p.Hq + head) * D;
       float* prow = p.part_o + (int64_t(part) * BM + t) * D;
       if (active) {
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld32(t_lane + uint32_t(TR::TM_O + c * 32), o);
+        for (int c = wg * (D / 32); c < (wg + 1) * (D / 32); ++c) {
+          uint32_t o[16];
+          tmem_ld16(t_lane + uint32_t(TR::TM_O + c * 16), o);
           tmem_wait_ld();
-          reg_fence32(o);
+          reg_fence16(o);
+          float f[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            f[e] = __uint_as_float(o[e]) * mult;
+            // e4m3 has no infinities: one in O stands for a NaN of V
+            if (TR::KV8 && (o[e] & 0x7FFFFFFFu) == 0x7F800000u) f[e] = __uint_as_float(0x7FC00000u);
+          }
           if (!valid) continue;
           if (whole) {
-            uint4* dst = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + orow * 2 + c * 64);
+            uint32_t h[8];
 #pragma unroll
-            for (int v4 = 0; v4 < 4; ++v4) {
-              uint32_t x[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float lo = __uint_as_float(o[v4 * 8 + 2 * i]) * mult, hi = __uint_as_float(o[v4 * 8 + 2 * i + 1]) * mult;
-                x[i] = p.out_bf16 ? pack_bf16x2(lo, hi) : pack_f16x2(lo, hi);
-              }
-              dst[v4] = make_uint4(x[0], x[1], x[2], x[3]);
-            }
+            for (int e = 0; e < 8; ++e)
+              h[e] = p.out_bf16 ? pack_bf16x2(f[2 * e], f[2 * e + 1]) : pack_f16x2(f[2 * e], f[2 * e + 1]);
+            uint4* dst = reinterpret_cast<uint4*>(out_row + c * 16);
+            dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+            dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
           } else {
-            float4* dst = reinterpret_cast<float4*>(prow + c * 32);
+            float4* dst = reinterpret_cast<float4*>(prow + c * 16);
 #pragma unroll
-            for (int v4 = 0; v4 < 8; ++v4)
-              dst[v4] = make_float4(__uint_as_float(o[4 * v4]) * mult, __uint_as_float(o[4 * v4 + 1]) * mult,
-                                    __uint_as_float(o[4 * v4 + 2]) * mult, __uint_as_float(o[4 * v4 + 3]) * mult);
+            for (int e = 0; e < 4; ++e) __stcg(dst + e, make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]));
           }
         }
       }
-      tc_fence_before();
-      mbar_arrive(o_free);
+      warp_arrive(o_free);
       if (valid) {
-        if (whole) {
-          p.lse[tok * p.Hq + head] = l == 0.f ? kNegInf : (ms + lg2_approx(l)) * kLn2;
-          if (sees_bad)
-            add_nonfinite<D>(p, r, seq, kvh, tok, node, 0, r.len, Add16{static_cast<uint16_t*>(p.out) + orow, p.out_bf16});
-        } else {
-          p.part_ml[part * BM + t] = make_float2(ms, l);
-          if (sees_bad) add_nonfinite<D>(p, r, seq, kvh, tok, node, kt0 * BN, (kt0 + n) * BN, AddF32{prow});
+        const float ms = m == kNegInf ? kNegInf : m * scale;  // log2 units
+        if (wg == 0) {
+          if (whole) p.lse[tok * p.Hq + head] = l == 0.f ? kNegInf : (ms + lg2_approx(l)) * kLn2;
+          else __stcg(&p.part_ml[part * BM + t], make_float2(ms, l));
         }
+        if (sees_bad)
+          add_nonfinite<D>(p, x.seq, x.kvh, ctx, x.lim, tok, node, x.kt0 * BN, (x.kt0 + n) * BN, wg * (D / 2),
+                           out_row, whole ? nullptr : prow);
       }
-      if (t == 0 && left_after <= 0) {
-        // the share's last item: if it began here and goes on, this CTA's descriptor names it
-        int4 d0 = make_int4(0, 0, 0, 0), d1 = d0;
-        if (begins && !whole) {
-          const int64_t end = share.t1 + (r.kt - n);  // one past the item's last tile
-          const int64_t g = min(int64_t(G), share.total);
-          d0 = make_int4(1, int((end * g - 1) / share.total), rows, mtile * BM);
-          d1 = make_int4(r.token0, kvh, 0, 0);
-        }
-        p.desc[2 * cta] = d0;
-        p.desc[2 * cta + 1] = d1;
+      if (threadIdx.x == 0 && !more && x.kt0 == 0 && !whole) {
+        // the share's last item began here and goes on: this CTA's descriptor names it, and the
+        // CTA that its last tile belongs to
+        p.desc[2 * cta] = make_int4(1, share.owner(share.t1 + (x.kt - n) - 1), rows, x.mtile * BM);
+        p.desc[2 * cta + 1] = make_int4(x.token0, x.kvh, 0, 0);
       }
+      it0 += n;
+      ++item;
+      x = y;
     }
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, 512);
+  if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -898,10 +1188,10 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
   if (d0.x == 0) return;
   const int4 d1 = p.desc[2 * c + 1];
   const int parts = d0.y - c + 1;
-  auto slot = [&](int i) { return i == 0 ? 2 * c + 1 : 2 * (c + i); };
+  auto slot = [&](int i) { return (i == 0 ? 2 * c + 1 : 2 * (c + i)) * BM; };
   for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < d0.z; row += gridDim.y * 8) {
     float top = kNegInf;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i) * BM + row].x);
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i) + row].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     constexpr int E = D / 32;
@@ -910,9 +1200,9 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
 #pragma unroll 4
     for (int i = 0; i < parts; ++i) {
-      const float2 ml = p.part_ml[slot(i) * BM + row];
+      const float2 ml = p.part_ml[slot(i) + row];
       const float f = ml.x == kNegInf ? 0.f : ex2_approx(ml.x - top);
-      const float* src = p.part_o + (int64_t(slot(i)) * BM + row) * D;
+      const float* src = p.part_o + int64_t(slot(i) + row) * D;
       l = fmaf(ml.y, f, l);
 #pragma unroll
       for (int e = 0; e < E; e += 2) {
@@ -924,8 +1214,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
       }
     }
     const int packed = d0.w + row, node = packed / p.group;
-    const int head = d1.y * p.group + (packed - node * p.group);
-    const int64_t o = (int64_t(d1.x) + node) * p.Hq + head;
+    const int64_t o = (int64_t(d1.x) + node) * p.Hq + d1.y * p.group + (packed - node * p.group);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     uint32_t* out = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(p.out) + o * D);
 #pragma unroll
@@ -963,10 +1252,10 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// Pool view [pages, page_size, heads, D] with a box of (128 bytes | an e4m3 row, 1 head,
-// `rows` rows, 1 page).
+// Pool view [pages, page_size, heads, D] with a box of (`inner` elements, 1 head, `rows` rows,
+// 1 page), swizzled over `swizzle` bytes (0: not).
 int make_pool_map(CUtensorMap* map, const void* base, int num_pages, int page_size, int heads, int D,
-                  int elem, const int64_t* strides, int rows) {
+                  int elem, const int64_t* strides, int rows, int inner, int swizzle) {
   static EncodeTiledFn enc = nullptr;
   if (enc == nullptr) {
     void* ptr = nullptr;
@@ -980,11 +1269,13 @@ int make_pool_map(CUtensorMap* map, const void* base, int num_pages, int page_si
                               cuuint64_t(num_pages > 0 ? num_pages : 1)};
   const cuuint64_t st[3] = {cuuint64_t(strides[2]) * elem, cuuint64_t(strides[1]) * elem,
                             cuuint64_t(strides[0]) * elem};
-  const cuuint32_t box[4] = {cuuint32_t(elem == 1 ? D : 64), 1, cuuint32_t(rows), 1};
+  const cuuint32_t box[4] = {cuuint32_t(inner), 1, cuuint32_t(rows), 1};
   const cuuint32_t es[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, elem == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 4,
                          const_cast<void*>(base), dims, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                         elem == 1 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B,
+                         swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                         : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                         : CU_TENSOR_MAP_SWIZZLE_NONE,
                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_last_error("cuTensorMapEncodeTiled (pool) failed (%d)", int(r));
@@ -1011,8 +1302,13 @@ int launch_tree(const void* k_pages, const void* v_pages, const int64_t* ks, con
   const int rows = p.page_size < TR::BN ? p.page_size : TR::BN;
   const int el = TR::KV8 ? 1 : 2;
   CUtensorMap mk, mv;
-  if (int rc = make_pool_map(&mk, p.num_pages ? k_pages : p.q, p.num_pages, p.page_size, p.Hkv, TR::D, el, ks, rows)) return rc;
-  if (int rc = make_pool_map(&mv, p.num_pages ? v_pages : p.q, p.num_pages, p.page_size, p.Hkv, TR::D, el, vs, rows)) return rc;
+  const void* none = p.q;  // an empty pool: every page is outside, nothing is read
+  if (int rc = make_pool_map(&mk, p.num_pages ? k_pages : none, p.num_pages, p.page_size, p.Hkv, TR::D, el, ks,
+                             rows, TR::K_SWZ / el, TR::K_SWZ))
+    return rc;
+  if (int rc = make_pool_map(&mv, p.num_pages ? v_pages : none, p.num_pages, p.page_size, p.Hkv, TR::D, el, vs,
+                             rows, TR::KV8 ? TR::D : 64, TR::KV8 ? 0 : 128))
+    return rc;
   tree_attn_kernel<TR><<<grid, TR::THREADS, TR::SMEM_BYTES, st>>>(mk, mv, p);
   if (int rc = check_launch("attn_fwd_paged_tree")) return rc;
   const int64_t most = int64_t(max_seqlen_q) * p.group;  // rows of a row tile
@@ -1051,7 +1347,8 @@ extern "C" int fa4cp_attn_fwd_paged_tree(
   const bool q8 = q_dtype == FA4CP_DTYPE_E4M3, kv8 = kv_dtype == FA4CP_DTYPE_E4M3;
   FA4CP_CHECK_ARG(q8 || q_dtype == FA4CP_DTYPE_BF16 || q_dtype == FA4CP_DTYPE_F16,
                   "q dtype must be f16, bf16 or e4m3");
-  FA4CP_CHECK_ARG(kv8 || kv_dtype == q_dtype, "K/V dtype must be e4m3 or the dtype of q");
+  FA4CP_CHECK_ARG(kv_dtype == q_dtype || (kv8 && q_dtype == FA4CP_DTYPE_BF16),
+                  "K/V dtype must be the dtype of q, or e4m3 under a bf16 q");
   FA4CP_CHECK_ARG(q8 || !q_descale, "q_descale applies to an e4m3 q only");
   FA4CP_CHECK_ARG(kv8 || (!k_descale && !v_descale), "descales apply to e4m3 K/V only");
   FA4CP_CHECK_ARG(softmax_scale > 0.f, "softmax_scale must be positive");
@@ -1109,11 +1406,11 @@ extern "C" int fa4cp_attn_fwd_paged_tree(
     return launch_tree<decltype(tr)>(k_pages, v_pages, k_strides, v_strides, max_seqlen_q, p, st);
   };
   if (kv8) {
-    if (head_dim == 64) return go(TreeTraits<64, 128, true>{});
-    if (head_dim == 128) return go(TreeTraits<128, 128, true>{});
-    return go(TreeTraits<256, 64, true>{});
+    if (head_dim == 64) return go(TreeTraits<64, true>{});
+    if (head_dim == 128) return go(TreeTraits<128, true>{});
+    return go(TreeTraits<256, true>{});
   }
-  if (head_dim == 64) return go(TreeTraits<64, 128, false>{});
-  if (head_dim == 128) return go(TreeTraits<128, 128, false>{});
-  return go(TreeTraits<256, 64, false>{});
+  if (head_dim == 64) return go(TreeTraits<64, false>{});
+  if (head_dim == 128) return go(TreeTraits<128, false>{});
+  return go(TreeTraits<256, false>{});
 }

@@ -65,8 +65,11 @@ def attn(q, k_pages, v_pages, table, cu, lens, seen, scale, kd=None, vd=None, qd
     fp32, so a score errs by at most e = (D + 8) 2^-24 sum|q||k| scale (and a P by a factor
     1 + 2e, with 2^-20 for the hardware exponential); P is rounded once to the 16-bit operand
     type (half a step u_p relative, 2^-25 absolute for an f16 that is subnormal), O is summed
-    in fp32, and out is rounded once (u_o).  An e4m3 cache is attended in f16, whose q is
-    scaled by a power of two to keep its largest value normal: 2^-24 of the row's largest.
+    in fp32, and out is rounded once (u_o).  Over an e4m3 cache P is an f16, and a bf16 q is
+    two e4m3 terms of q 2^s with the row's largest in [2^7, 2^8): the first leaves at most half
+    of its last place, the second holds that exactly but for what is below half of the least
+    e4m3, 2^-10, so q errs by at most 2^-17 of the row's largest.  The descales and the
+    scales of the operands add a few roundings in fp32.
     """
     T, H, D = q.shape
     hk = k_pages.shape[2]
@@ -108,11 +111,11 @@ def attn(q, k_pages, v_pages, table, cu, lens, seen, scale, kd=None, vd=None, qd
                 A = w[i, ii] @ vv[ii].abs()
                 e = (D + 8) * 2.0 ** -24 * scale * float(
                     ((kk[ii].abs() @ x[i].abs()).max() if ii.any() else 0.0))
-                if kv8:
-                    e += 2.0 ** -24 * scale * float(x[i].abs().max()) * float(
+                if kv8 and q.dtype != E4M3:
+                    e += 2.0 ** -17 * scale * float(x[i].abs().max()) * float(
                         kk[ii].abs().sum(1).max() if ii.any() else 0.0)
                 m = int(ii.sum())
-                rel = u_p + 2 * (2 * e + 2.0 ** -20) + m * 2.0 ** -24
+                rel = u_p + 2 * (2 * e + 2.0 ** -20) + (m + 8) * 2.0 ** -24
                 low = m * 2.0 ** -25 * (vv[ii].abs().max(0).values if m else 0.0) \
                     if (kv8 or q.dtype == torch.float16) else 0.0
                 tol[a + i, h] = rel * A + low + u_o * (A + out[a + i, h].abs()) + 2.0 ** -25
