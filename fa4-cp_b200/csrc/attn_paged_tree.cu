@@ -26,7 +26,8 @@
 //               elected lane each: an issuer is held up while the tensor core is busy, so the
 //               waits of one hide behind the other's MMAs)
 //   warps 12-15 e4m3 cache only: V tiles from a raw ring, widened to f16
-// TMEM: 4 S buffers (64 fp32 columns each, 32 at head_dim 256) | O (D columns) | Q (D/2).
+// TMEM: S buffers (64 fp32 columns each, 32 at head_dim 256) | O (D columns, twice up to
+// head_dim 128) | Q (D/2).
 // P(j) lies over S(j), as 16-bit pairs, and is the A operand of O += P V; S(j + buffers) waits
 // for PV(j).  A hand-over between two roles takes 200 to 300 cycles, and a tile has five of
 // them, so it is the number of tiles in flight that counts: four of 64 keys ran 1.5 times as
@@ -36,9 +37,11 @@
 // An e4m3 cache: K is multiplied as it is, by a Q in two e4m3 terms (hi + lo of q x 2^s, which
 // hold a bf16 to 2^-17 of its row's largest value), at twice the rate a term; V is widened to
 // f16, because a P in e4m3 would have to be two terms as well, at three conversions a value.
-// The warpgroups share one running maximum a row, handed from tile to tile through shared
-// memory right after a tile's maximum is known (its exponentials come later), and each keeps
-// its own row sum; so one warpgroup's exponentials overlap the other's waits and maxima.
+// Up to head_dim 128 the warpgroups work apart, each with an O, a running maximum and a sum of
+// its own, joined when the item ends: handing one maximum from tile to tile made every tile wait
+// for the one before (e4m3, head_dim 64, 64 tokens: 486 us, apart 324; one token: 203 and 157).
+// TMEM has no room for that at head_dim 256; there they share one O and one maximum a row, handed
+// on through shared memory right after a tile's maximum is known (its exponentials come later).
 // What runs once an item is written as small loops: its instructions come from L2 each time.
 #include <atomic>
 
@@ -125,7 +128,8 @@ struct TreeTraits {
   // k_full, k_empty [KS]; v_full, v_empty [VS]; r_full, r_empty [RS]; s_full, p_full, o_done
   // [NB]; max_known[8] (warpgroup, warp), v_fixed[2], q_full, o_free, joined, teardown;
   // q_staged, item_full, item_free [kItems]
-  static constexpr int NB = 4;  // S buffers
+  static constexpr bool APART = D <= 128;
+  static constexpr int NB = D == 128 ? 3 : 4;  // S buffers: what TMEM leaves
   static constexpr int NUM_BARS = 2 * (KS + VS + RS) + 3 * NB + 14 + 3 * kItems;
   // q_staged(i) is waited for before q_staged(i + kItems) can complete: the items between them
   // take two slots of the K ring each, so the latter needs the former's slots back
@@ -140,7 +144,7 @@ struct TreeTraits {
   static constexpr int REGS_SOFTMAX = KV8 ? 168 : 184, REGS_CONTROL = KV8 ? 80 : 136, REGS_CONV = 96;
   static_assert(128 * (2 * REGS_SOFTMAX + REGS_CONTROL) + 32 * CONV_WARPS * REGS_CONV <=
                     (KV8 ? 512 * 128 : 384 * 168), "register split exceeds the launch allocation");
-  static constexpr int TM_S = 0, TM_O = NB * BN, TM_Q = TM_O + D;
+  static constexpr int TM_S = 0, TM_O = NB * BN, TM_Q = TM_O + (APART ? 2 : 1) * D;
   static_assert(TM_Q + D / 2 <= 512, "TMEM budget");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
@@ -806,8 +810,8 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys: 16 rows of 128 bytes further
-                mma_f16_ts(tmem + TR::TM_O, tmem + uint32_t(TR::TM_S + kk * 8) + it % NB * BN, desc + uint64_t(kk * 16 * 128 / 16),
-                           idesc, (j > 0 || kk > 0) ? 1u : 0u);
+                mma_f16_ts(tmem + TR::TM_O + (TR::APART ? (it & 1) * D : 0u), tmem + uint32_t(TR::TM_S + kk * 8) + it % NB * BN,
+                           desc + uint64_t(kk * 16 * 128 / 16), idesc, (j > (TR::APART ? 1 : 0) || kk > 0) ? 1u : 0u);
               tc_commit(o_done(it));
               tc_commit(v_empty(it));
             }
@@ -827,6 +831,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
     const int wg = warp >> 2, w4 = warp & 3;
     const int t = threadIdx.x & 127;  // row of the tile
     const uint32_t t_lane = tmem + (uint32_t(w4 * 32) << 16);
+    const uint32_t t_o = t_lane + uint32_t(TR::TM_O + (TR::APART ? wg * D : 0));
     const bool bf16_op = p.kv_dtype == FA4CP_DTYPE_BF16;
     const bool q8 = p.q_dtype == FA4CP_DTYPE_E4M3;
     // One arrival a warp, for its lanes' TMEM (and shared memory) accesses so far.
@@ -936,8 +941,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         scale /= qf;
         scale = scale < 1.17549435e-38f ? 1.17549435e-38f : scale;
       }
-      // m: the maximum that O and this warpgroup's sum l are relative to, as far as this
-      // warpgroup knows
+      // m: the maximum that this warpgroup's sum l (and its O) are relative to
       float m = kNegInf, l = 0.f;
       bool sees_bad = false;
       for (int j = (it0 & 1) == uint32_t(wg) ? 0 : 1; j < n; j += 2) {
@@ -982,34 +986,41 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
               for (int k = 0; k < 4; ++k)
                 mx4[k] = fmax3(mx4[k], __uint_as_float(sr[c][e + 2 * k]), __uint_as_float(sr[c][e + 2 * k + 1]));
           const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-          if (!max_settled()) { aborted = true; break; }
+          // the maximum is raised only when it would grow by more than 2^8, or comes to exist
           float so_far = kNegInf;
-          if (j > 0) so_far = row_max[t];
-          // raised only when it would grow by more than 2^8, or comes to exist
-          const bool need = j > 0 && (so_far == kNegInf ? mx != kNegInf : (mx - so_far) * scale > kRescaleThreshold);
-          const float m_new = need || j == 0 ? mx : so_far;
-          row_max[t] = m_new;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(max_known(wg, w4));
+          if constexpr (TR::APART) {
+            so_far = m;
+          } else {
+            if (!max_settled()) { aborted = true; break; }
+            if (j > 0) so_far = row_max[t];
+          }
+          const bool raise = so_far == kNegInf ? mx != kNegInf : (mx - so_far) * scale > kRescaleThreshold;
+          const float m_new = raise ? mx : so_far;
+          if constexpr (!TR::APART) {
+            row_max[t] = m_new;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(max_known(wg, w4));
+          }
           // from here on off the other warpgroup's way
           if (m_new != m) {
             if (m != kNegInf) l *= ex2_approx((m - m_new) * scale);
             m = m_new;
           }
-          if (__any_sync(0xffffffffu, need)) {
-            const float f = !need ? 1.f : so_far == kNegInf ? 0.f : ex2_approx((so_far - m_new) * scale);
-            ok = mbar_wait(o_done(it - 1), phase(it - 1, NB), abort, kErrODone, status);
+          constexpr int MINE = TR::APART ? 2 : 1;  // PV(it - MINE) was the last one into this O
+          if (j >= MINE && __any_sync(0xffffffffu, raise)) {
+            const float f = !raise ? 1.f : so_far == kNegInf ? 0.f : ex2_approx((so_far - m_new) * scale);
+            ok = mbar_wait(o_done(it - MINE), phase(it - MINE, NB), abort, kErrODone, status);
             if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D / 16; ++c) {
               uint32_t o[16];
-              tmem_ld16(t_lane + uint32_t(TR::TM_O + c * 16), o);
+              tmem_ld16(t_o + uint32_t(c * 16), o);
               tmem_wait_ld();
               reg_fence16(o);
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st16(t_lane + uint32_t(TR::TM_O + c * 16), o);
+              tmem_st16(t_o + uint32_t(c * 16), o);
             }
           }
           const float neg_m = (m == kNegInf) ? 0.f : -m * scale;
@@ -1029,7 +1040,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           for (int c = 0; c < C; ++c) tmem_st16(t_s + uint32_t(c * 16), pw[c]);
           const uint64_t rsum = fadd2(rs[0], rs[1]);
           l += f2lo(rsum) + f2hi(rsum);
-        } else {
+        } else if (!TR::APART) {
           if (!max_settled()) { aborted = true; break; }
           if (lane == 0) mbar_arrive(max_known(wg, w4));
         }
@@ -1102,15 +1113,20 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       if (ok) ok = mbar_wait(o_done(last), phase(last, NB), abort, kErrODone, status);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      // the last tile's warpgroup knows the maximum that O is relative to
-      m = end_max[(set + int(last & 1)) * BM + t];
+      // Apart: O = f0 O0 + f1 O1.  Shared: O is relative to the last tile's maximum.
+      float part_max[2], part_f[2];
+#pragma unroll
+      for (int g = 0; g < 2; ++g) part_max[g] = end_max[(set + g) * BM + t];
+      m = TR::APART ? fmaxf(part_max[0], part_max[1]) : part_max[last & 1];
       l = 0.f;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        const float mg = end_max[(set + g) * BM + t], lg = end_sum[(set + g) * BM + t];
-        l += mg == m || mg == kNegInf ? lg : lg * ex2_approx((mg - m) * scale);
+        const float lg = end_sum[(set + g) * BM + t];
+        part_f[g] = part_max[g] == m ? 1.f : part_max[g] == kNegInf ? 0.f : ex2_approx((part_max[g] - m) * scale);
+        l += part_max[g] == kNegInf ? lg : lg * part_f[g];  // (NaN sums have no maximum)
         sees_bad |= end_bad[(set + g) * BM + t] != 0;
       }
+      const bool two = TR::APART && n > 1;  // the last tile's O, and the other one
       const bool whole = n == x.kt;
       const int part = 2 * cta + (x.kt0 == 0 ? 1 : 0);
       const float mult = whole ? (l == 0.f ? 0.f : vscale / l) : vscale;
@@ -1119,13 +1135,21 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       if (active) {
 #pragma unroll 1
         for (int c = wg * (D / 32); c < (wg + 1) * (D / 32); ++c) {
-          uint32_t o[16];
-          tmem_ld16(t_lane + uint32_t(TR::TM_O + c * 16), o);
+          uint32_t o[16], o2[16];
+          const uint32_t from = t_lane + uint32_t(TR::TM_O + c * 16);
+          tmem_ld16(from + (TR::APART ? (last & 1) * D : 0u), o);
+          if (two) tmem_ld16(from + (~last & 1) * D, o2);
           tmem_wait_ld();
           reg_fence16(o);
+          reg_fence16(o2);
           float f[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
+            if (TR::APART) {
+              float y = __uint_as_float(o[e]) * part_f[last & 1];
+              if (two) y = fmaf(__uint_as_float(o2[e]), part_f[~last & 1], y);
+              o[e] = __float_as_uint(y);
+            }
             f[e] = __uint_as_float(o[e]) * mult;
             // e4m3 has no infinities: one in O stands for a NaN of V
             if (TR::KV8 && (o[e] & 0x7FFFFFFFu) == 0x7F800000u) f[e] = __uint_as_float(0x7FC00000u);
