@@ -260,62 +260,124 @@ struct WriteParams {
   Pool kp, vp;
   const int64_t* slots;
   int64_t tokens, num_slots;
-  int heads, per_head, page_size;  // per_head: 16-byte chunks of a stored head row
+  int heads, per_head, page_size;  // per_head: 16-byte pieces of a head's source row
 };
 
-template <bool BF16>
-__device__ __forceinline__ uint4 quant16(const uint4 a, const uint4 b, float d) {
-  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float f[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t x = w[2 * i + h];
-      if (BF16) {
-        f[2 * h] = __uint_as_float(x << 16);
-        f[2 * h + 1] = __uint_as_float(x & 0xFFFF0000u);
-      } else {
-        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&x));
-        f[2 * h] = t.x;
-        f[2 * h + 1] = t.y;
-      }
-    }
-    // one rounding, of the quotient: a multiplication by 1 / d would round twice
-    o[i] = pack_e4m3x4(__fdiv_rn(f[0], d), __fdiv_rn(f[1], d), __fdiv_rn(f[2], d), __fdiv_rn(f[3], d));
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
+// The divisor of a head's values.  Every value needs the rounded quotient x / d, since e4m3 of
+// x * (1 / d) would round twice; but the reciprocal is the same for all of them, and a quotient
+// from a correctly rounded reciprocal needs one correction (P. Markstein, IBM J. Res. Dev. 34,
+// 1990): q = x r, q + r (x - q d).  The remainder is a normal number, or 0, wherever the result
+// is not 0 in e4m3, as long as |d| is between 2^-60 and 2^60; other divisors are brought there
+// by a power of two, and the values by the same.  (A quotient costs three products, the
+// division about ten instructions.)
+struct Divisor {
+  float d, r, scale;
+};
+
+__device__ __forceinline__ Divisor divisor(const float* descale, int head) {
+  Divisor v;
+  const float d = descale ? descale[head] : 1.f, a = fabsf(d);
+  v.scale = a < 0x1p-60f ? 0x1p100f : a > 0x1p60f ? 0x1p-100f : 1.f;
+  v.d = d * v.scale;
+  v.r = __frcp_rn(v.d);
+  if (isinf(d)) v.d = 1.f;  // r = 0: all quotients are 0, those of infinities NaN
+  return v;
 }
 
-// One thread per 16 bytes stored in K and in V.  QUANT: 0 copy, 1 bf16 -> e4m3, 2 f16 -> e4m3.
-template <int QUANT>
-__global__ void __launch_bounds__(256) kv_write_kernel(const WriteParams p) {
-  const unsigned per_head = unsigned(p.per_head);
-  const unsigned per_row = per_head * unsigned(p.heads);
-  const int64_t n = p.tokens * per_row;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < n;
-       i += int64_t(gridDim.x) * blockDim.x) {
-    const int64_t t = n < (int64_t(1) << 32) ? int64_t(uint32_t(i) / per_row) : i / per_row;
-    const unsigned c = unsigned(i - t * per_row);
-    const int64_t slot = p.slots[t];
-    if (slot < 0 || slot >= p.num_slots) continue;
-    const unsigned head = c / per_head, x = c - head * per_head;
-    const int64_t page = slot / p.page_size, row = slot - page * p.page_size;
-    const uint8_t* ks = p.k + t * p.k_stride + int64_t(c) * (QUANT ? 32 : 16);
-    const uint8_t* vs = p.v + t * p.v_stride + int64_t(c) * (QUANT ? 32 : 16);
-    uint4 ko, vo;
-    if (QUANT) {
-      const uint4 k0 = __ldcs(reinterpret_cast<const uint4*>(ks)), k1 = __ldcs(reinterpret_cast<const uint4*>(ks) + 1);
-      const uint4 v0 = __ldcs(reinterpret_cast<const uint4*>(vs)), v1 = __ldcs(reinterpret_cast<const uint4*>(vs) + 1);
-      ko = quant16<QUANT == 1>(k0, k1, p.k_descale ? p.k_descale[head] : 1.f);
-      vo = quant16<QUANT == 1>(v0, v1, p.v_descale ? p.v_descale[head] : 1.f);
+// Eight values, stored as eight bytes.
+template <bool BF16>
+__device__ __forceinline__ uint2 quant8(const uint4 a, const Divisor& d) {
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+  // with the signs of a product x (-1 / d), which keep that of a zero
+  const uint64_t scale = f2pack(-d.scale, -d.scale), r = f2pack(-d.r, -d.r), dd = f2pack(d.d, d.d);
+  float q[8], f[8], top[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint64_t x;
+    if (BF16) {
+      x = f2pack(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
     } else {
-      ko = __ldcs(reinterpret_cast<const uint4*>(ks));
-      vo = __ldcs(reinterpret_cast<const uint4*>(vs));
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x = f2pack(t.x, t.y);
     }
-    *reinterpret_cast<uint4*>(p.kp.base + page * p.kp.page + row * p.kp.row + head * p.kp.head + x * 16) = ko;
-    *reinterpret_cast<uint4*>(p.vp.base + page * p.vp.page + row * p.vp.row + head * p.vp.head + x * 16) = vo;
+    x = fmul2(x, scale);
+    const uint64_t y = fmul2(x, r);
+    q[2 * i] = f2lo(y);
+    q[2 * i + 1] = f2hi(y);
+    const uint64_t c = ffma2(ffma2(y, dd, x), r, y);
+    f[2 * i] = f2lo(c);
+    f[2 * i + 1] = f2hi(c);
+    top[i] = fmaxf(fabsf(q[2 * i]), fabsf(q[2 * i + 1]));
+  }
+  if (fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) > 4096.f) {
+    // what saturates may be infinite, and leave no remainder to add
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = fabsf(q[i]) > 4096.f ? q[i] : f[i];
+  }
+  return make_uint2(pack_e4m3x4(f[0], f[1], f[2], f[3]), pack_e4m3x4(f[4], f[5], f[6], f[7]));
+}
+
+constexpr int kWriteThreads = 256, kWriteBlocks = 4, kWriteBatch = 2;
+
+// A thread owns 16 bytes of the source row's columns, in K and in V, and takes a token out of
+// every `gridDim.x` groups of them.  QUANT: 0 copy, 1 bf16 -> e4m3, 2 f16 -> e4m3.  Bound by
+// memory: a row's loads do not wait for its slot, which decides on the store alone.  Measured:
+// 65536 rows of 8 heads x 128, bf16 into e4m3, 73.5 us = 5.5 TB/s (62.4 us at the rate of a
+// copy); a thread a token instead of the loop 93 us, batches of 4 at 64 registers (spills) 86 us,
+// at 80 registers (3 blocks) 77 us.  64 rows: 1.7 us, the launch.
+template <int QUANT>
+__global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(const WriteParams p) {
+  const int cols = min(p.heads * p.per_head, kWriteThreads);  // of a block
+  const int group = kWriteThreads / cols;                     // its tokens
+  const int c = int(blockIdx.y) * cols + int(threadIdx.x) % cols;
+  const int in_group = int(threadIdx.x) / cols;
+  if (in_group >= group || c >= p.heads * p.per_head) return;
+  const int head = c / p.per_head, x = c - head * p.per_head;
+  const int64_t step = int64_t(gridDim.x) * group;
+  constexpr int OUT = QUANT ? 8 : 16;
+  const uint8_t *ks = p.k + int64_t(c) * 16, *vs = p.v + int64_t(c) * 16;
+  uint8_t* kd = p.kp.base + head * p.kp.head + x * OUT;
+  uint8_t* vd = p.vp.base + head * p.vp.head + x * OUT;
+  Divisor dk, dv;
+  if (QUANT) {
+    dk = divisor(p.k_descale, head);
+    dv = divisor(p.v_descale, head);
+  }
+  for (int64_t t0 = int64_t(blockIdx.x) * group + in_group; t0 < p.tokens; t0 += step * kWriteBatch) {
+    uint4 k[kWriteBatch], v[kWriteBatch];
+    int64_t slot[kWriteBatch];
+#pragma unroll
+    for (int i = 0; i < kWriteBatch; ++i) {
+      const int64_t t = t0 + i * step;
+      slot[i] = -1;
+      if (t < p.tokens) {
+        slot[i] = p.slots[t];
+        k[i] = __ldcs(reinterpret_cast<const uint4*>(ks + t * p.k_stride));
+        v[i] = __ldcs(reinterpret_cast<const uint4*>(vs + t * p.v_stride));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kWriteBatch; ++i) {
+      if (slot[i] < 0 || slot[i] >= p.num_slots) continue;
+      int64_t page, row;
+      if (p.num_slots < (int64_t(1) << 32)) {
+        const uint32_t g = uint32_t(slot[i]) / uint32_t(p.page_size);
+        page = g;
+        row = uint32_t(slot[i]) - g * uint32_t(p.page_size);
+      } else {
+        page = slot[i] / p.page_size;
+        row = slot[i] - page * p.page_size;
+      }
+      uint8_t* ko = kd + page * p.kp.page + row * p.kp.row;
+      uint8_t* vo = vd + page * p.vp.page + row * p.vp.row;
+      if (QUANT) {
+        *reinterpret_cast<uint2*>(ko) = quant8<QUANT == 1>(k[i], dk);
+        *reinterpret_cast<uint2*>(vo) = quant8<QUANT == 1>(v[i], dv);
+      } else {
+        *reinterpret_cast<uint4*>(ko) = k[i];
+        *reinterpret_cast<uint4*>(vo) = v[i];
+      }
+    }
   }
 }
 
@@ -332,11 +394,12 @@ struct AcceptParams {
   int num_pages, page_size, max_pages, max_accept, heads, per_head;  // per_head: 16-byte chunks
 };
 
-// CTA = (request, share of the row's 16-byte columns).  A thread owns a column of K or of V
-// through all moved rows.  The list ascends, so node a_i >= i: a batch of loads followed by
-// its stores never overwrites a row that a later batch reads.
+// CTA = (request, share of the row's 16-byte columns).  The moves (page and row that each comes
+// from and goes to) are worked out once, a thread each; then a thread owns a column of K or of V
+// through all of them.  The list ascends, so node a_i >= i: a batch of loads followed by its
+// stores never overwrites a row that a later batch reads.
 __global__ void __launch_bounds__(kAcceptThreads) kv_accept_kernel(const AcceptParams p) {
-  extern __shared__ int s_pos[];  // [max_accept]: node, or -1 where nothing moves
+  extern __shared__ int4 s_move[];  // [max_accept]: from (page, row), to (page, row); page -1: stays
   __shared__ int s_n;
   const int j = blockIdx.x, lane = threadIdx.x & 31;
   const int base = max(p.cached[j], 0);
@@ -351,7 +414,7 @@ __global__ void __launch_bounds__(kAcceptThreads) kv_accept_kernel(const AcceptP
       const bool good = a > before && a >= 0 && a < nodes;
       const unsigned bad = __ballot_sync(0xffffffffu, !good);
       const int run = bad ? __ffs(bad) - 1 : 32;
-      if (lane < run) s_pos[i] = a;
+      if (lane < run) s_move[i].x = a;
       n += run;
       if (run < 32) break;
       last = __shfl_sync(0xffffffffu, a, 31);
@@ -363,17 +426,24 @@ __global__ void __launch_bounds__(kAcceptThreads) kv_accept_kernel(const AcceptP
   }
   __syncthreads();
   const int n = s_n;
+  const int32_t* table = p.table + int64_t(j) * p.max_pages;
+  for (int i = threadIdx.x; i < n; i += kAcceptThreads) {
+    const int a = s_move[i].x;
+    auto place = [&](int node, int& page, int& row) {
+      const unsigned pos = unsigned(base) + unsigned(node);  // below 2^32
+      const unsigned e = pos / unsigned(p.page_size);
+      page = e < unsigned(p.max_pages) ? table[e] : -1;
+      row = int(pos - e * unsigned(p.page_size));
+      if (page >= p.num_pages) page = -1;
+    };
+    int4 m;
+    place(a, m.x, m.y);
+    place(i, m.z, m.w);
+    if (a == i || m.x < 0 || m.z < 0) m.x = -1;
+    s_move[i] = m;
+  }
+  __syncthreads();
   const int cols = p.heads * p.per_head;
-  const int32_t* row = p.table + int64_t(j) * p.max_pages;
-  auto offset = [&](const Pool& pool, int node, int64_t& off) -> bool {
-    const int64_t pos = int64_t(base) + node;
-    const int64_t e = pos / p.page_size;
-    if (e >= p.max_pages) return false;
-    const int page = row[e];
-    if (page < 0 || page >= p.num_pages) return false;
-    off = int64_t(page) * pool.page + (pos - e * p.page_size) * pool.row;
-    return true;
-  };
   for (int u = blockIdx.y * kAcceptThreads + threadIdx.x; u < 2 * cols; u += gridDim.y * kAcceptThreads) {
     const Pool pool = u < cols ? p.kp : p.vp;
     const int c = u < cols ? u : u - cols;
@@ -381,17 +451,17 @@ __global__ void __launch_bounds__(kAcceptThreads) kv_accept_kernel(const AcceptP
     uint8_t* col = pool.base + head * pool.head + int64_t(c - head * p.per_head) * 16;
     for (int i0 = 0; i0 < n; i0 += 8) {
       uint4 x[8];
-      bool ok[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        int64_t off = 0;
-        ok[i] = i0 + i < n && s_pos[i0 + i] != i0 + i && offset(pool, s_pos[i0 + i], off);
-        if (ok[i]) x[i] = *reinterpret_cast<const uint4*>(col + off);
+        if (i0 + i >= n) break;
+        const int4 m = s_move[i0 + i];
+        if (m.x >= 0) x[i] = *reinterpret_cast<const uint4*>(col + m.x * pool.page + m.y * pool.row);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        int64_t off = 0;
-        if (ok[i] && offset(pool, i0 + i, off)) *reinterpret_cast<uint4*>(col + off) = x[i];
+        if (i0 + i >= n) break;
+        const int4 m = s_move[i0 + i];
+        if (m.x >= 0) *reinterpret_cast<uint4*>(col + m.z * pool.page + m.w * pool.row) = x[i];
       }
     }
   }
@@ -502,15 +572,21 @@ extern "C" int fa4cp_paged_kv_write(const void* k, const void* v, int64_t k_toke
   p.tokens = num_tokens;
   p.num_slots = num_pages * page_size;
   p.heads = num_heads_kv;
-  p.per_head = head_dim * pe / 16;
+  p.per_head = head_dim * se / 16;
   p.page_size = page_size;
-  const int64_t n = num_tokens * num_heads_kv * p.per_head;
-  const int64_t blocks = (n + 255) / 256;
-  const unsigned grid = unsigned(blocks < (int64_t(1) << 30) ? blocks : (int64_t(1) << 30));
+  const int64_t columns = int64_t(num_heads_kv) * p.per_head;
+  FA4CP_CHECK_ARG(columns < (int64_t(1) << 24), "rows of %lld bytes are too long", (long long)columns * 16);
+  const int cols = int(columns < kWriteThreads ? columns : kWriteThreads);
+  const int64_t groups = (num_tokens + kWriteThreads / cols - 1) / (kWriteThreads / cols);
+  const int64_t parts = (columns + cols - 1) / cols;
+  // a token a thread while that fills the SMs; beyond it, as many blocks as are resident, since
+  // what a thread works out once (its head, the divisor) then serves many tokens
+  const int64_t most = (kMaxGrid * kWriteBlocks + parts - 1) / parts;
+  const dim3 grid(unsigned(groups < most ? groups : most), unsigned(parts));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!quant) kv_write_kernel<0><<<grid, 256, 0, st>>>(p);
-  else if (src_dtype == FA4CP_DTYPE_BF16) kv_write_kernel<1><<<grid, 256, 0, st>>>(p);
-  else kv_write_kernel<2><<<grid, 256, 0, st>>>(p);
+  if (!quant) kv_write_kernel<0><<<grid, kWriteThreads, 0, st>>>(p);
+  else if (src_dtype == FA4CP_DTYPE_BF16) kv_write_kernel<1><<<grid, kWriteThreads, 0, st>>>(p);
+  else kv_write_kernel<2><<<grid, kWriteThreads, 0, st>>>(p);
   return check_launch("paged_kv_write");
 }
 
@@ -530,8 +606,10 @@ extern "C" int fa4cp_paged_kv_accept(void* k_pages, void* v_pages, const int64_t
   FA4CP_CHECK_ARG(head_dim * pe % 16 == 0, "a head's row must be a multiple of 16 bytes");
   FA4CP_CHECK_ARG(block_table && cached_lens && cu_q && seq_lens && k_strides && v_strides &&
                       (max_accept == 0 || accepted), "null tensor pointer");
-  if (int rc = check_pool("k_pages", k_pages, k_strides[0], k_strides[1], k_strides[2], pe)) return rc;
-  if (int rc = check_pool("v_pages", v_pages, v_strides[0], v_strides[1], v_strides[2], pe)) return rc;
+  if (num_pages > 0) {
+    if (int rc = check_pool("k_pages", k_pages, k_strides[0], k_strides[1], k_strides[2], pe)) return rc;
+    if (int rc = check_pool("v_pages", v_pages, v_strides[0], v_strides[1], v_strides[2], pe)) return rc;
+  }
   AcceptParams p{};
   p.kp = Pool{static_cast<uint8_t*>(k_pages), k_strides[0] * pe, k_strides[1] * pe, k_strides[2] * pe};
   p.vp = Pool{static_cast<uint8_t*>(v_pages), v_strides[0] * pe, v_strides[1] * pe, v_strides[2] * pe};
@@ -549,7 +627,7 @@ extern "C" int fa4cp_paged_kv_accept(void* k_pages, void* v_pages, const int64_t
   const int64_t cols = int64_t(2) * p.heads * p.per_head;
   const int64_t want = (cols + kAcceptThreads - 1) / kAcceptThreads;
   const dim3 grid(unsigned(nseq), unsigned(want < 64 ? want : 64));
-  kv_accept_kernel<<<grid, kAcceptThreads, size_t(max_accept > 0 ? max_accept : 1) * 4,
+  kv_accept_kernel<<<grid, kAcceptThreads, size_t(max_accept > 0 ? max_accept : 1) * 16,
                      static_cast<cudaStream_t>(stream)>>>(p);
   return check_launch("paged_kv_accept");
 }

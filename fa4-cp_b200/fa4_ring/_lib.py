@@ -180,7 +180,8 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def stream_of(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle alone: a torch.cuda.Stream object costs 2 us, as much as the launch
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 _no_switch = contextlib.nullcontext()
@@ -188,7 +189,7 @@ _no_switch = contextlib.nullcontext()
 
 def on_device(dev: torch.device):
     """Context in which launches go to ``dev`` (nothing to do when it is the current device)."""
-    return _no_switch if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _no_switch if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def ptr(t) -> int:
@@ -197,9 +198,7 @@ def ptr(t) -> int:
 
 def require_cuda(*tensors) -> None:
     for t in tensors:
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        if t is not None and (not isinstance(t, torch.Tensor) or not t.is_cuda):
             raise RuntimeError(
                 "fa4_ring (B200) runs on CUDA tensors only; got "
                 f"{'a CPU tensor' if isinstance(t, torch.Tensor) else type(t).__name__} "

@@ -13,6 +13,7 @@ one of the three zig-zag step patterns, addressing the row halves in place.
 """
 
 import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -48,6 +49,9 @@ def norm_descale(d: Optional[torch.Tensor], h_kv: int, device) -> Optional[torch
     ``[H_kv]`` CUDA tensor (fa4_ring/fa4_backend.py:45-55)."""
     if d is None:
         return None
+    if (torch.is_tensor(d) and d.dtype is torch.float32 and d.dim() == 1 and d.numel() == h_kv
+            and d.device == device and d.is_contiguous()):
+        return d
     if not torch.is_tensor(d):
         d = torch.tensor(float(d))
     d = d.to(device=device, dtype=torch.float32)
@@ -234,17 +238,22 @@ def b200_attn_paged(
 _Strides = ctypes.c_int64 * 3
 
 
+@functools.lru_cache(maxsize=256)
+def _strides_of(shape, stride, what: str):
+    n, rows, heads, d = shape
+    sp, sr, sh, sd = stride
+    if sd != 1:
+        raise ValueError(f"{what}: the last dimension must be contiguous")
+    return _Strides(sp if n > 1 else rows * heads * d, sr if rows > 1 else heads * d,
+                    sh if heads > 1 else d)
+
+
 def pool_strides(pool: torch.Tensor, what: str):
     """(page, row, head) strides, in elements, of a pool ``[pages, page, H_kv, D]``.  Any view
     with a dense last dimension is taken as it is; the library wants the strides in multiples
     of 16 bytes.  (A pool is never copied: a copy would double the cache, and a write into it
     would be lost.)"""
-    n, rows, heads, d = pool.shape
-    sp, sr, sh, sd = pool.stride()
-    if sd != 1:
-        raise ValueError(f"{what}: the last dimension must be contiguous")
-    return _Strides(sp if n > 1 else rows * heads * d, sr if rows > 1 else heads * d,
-                    sh if heads > 1 else d)
+    return _strides_of(pool.shape, pool.stride(), what)
 
 
 def rows16(x: torch.Tensor) -> torch.Tensor:
@@ -261,6 +270,11 @@ def as_i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
         return t
     return t.to(device=dev, dtype=torch.int32).contiguous()
+
+
+@functools.lru_cache(maxsize=64)
+def _tree_workspace_bytes(heads: int, heads_kv: int, dim: int, max_seqlen_q: int) -> int:
+    return max(_lib.load().fa4cp_attn_paged_tree_workspace_bytes(heads, heads_kv, dim, max_seqlen_q), 16)
 
 
 def b200_attn_paged_tree(
@@ -320,12 +334,11 @@ def b200_attn_paged_tree(
     q = rows16(q)
     ks, vs = pool_strides(k_pages, "k_pages"), pool_strides(v_pages, "v_pages")
     bt, cu, lens = as_i32(block_table, dev), as_i32(cu_seqlens_q, dev), as_i32(seq_lens, dev)
-    out = torch.empty((T, H, D), dtype=out_dtype_for(q.dtype), device=dev)
-    lse = torch.empty((T, H), dtype=torch.float32, device=dev)
+    out = q.new_empty((T, H, D), dtype=out_dtype_for(q.dtype))
+    lse = q.new_empty((T, H), dtype=torch.float32)
     lib = _lib.load()
     with _lib.on_device(dev):
-        ws_bytes = lib.fa4cp_attn_paged_tree_workspace_bytes(H, h_kv, D, max_seqlen_q)
-        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+        ws = q.new_empty(_tree_workspace_bytes(H, h_kv, D, max_seqlen_q), dtype=torch.uint8)
         rc = lib.fa4cp_attn_fwd_paged_tree(
             q.data_ptr(), q.stride(0), k_pages.data_ptr(), v_pages.data_ptr(), ks, vs,
             bt.data_ptr(), page_size, num_pages, bt.shape[1], out.data_ptr(), lse.data_ptr(),

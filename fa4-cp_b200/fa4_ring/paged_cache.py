@@ -44,8 +44,8 @@ class PagedPlan(NamedTuple):
     pages: torch.Tensor         # int32 [2]: pages taken from free_pages, pages not provided
 
 
-def _check_pools(k_pages, v_pages):
-    _lib.require_cuda(k_pages, v_pages)
+def _check_pools(k_pages, v_pages, *others):
+    _lib.require_cuda(k_pages, v_pages, *others)
     assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, "pools are [pages, page, H_kv, D]"
     assert k_pages.dtype == v_pages.dtype, "the pools must share a dtype"
     assert k_pages.device == v_pages.device, "the pools must be on one device"
@@ -93,11 +93,9 @@ def paged_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor,
         num_free = as_i32(num_free, dev)
         assert num_free.numel() == 1, "num_free is one number"
     cached_lens, new_lens, free_pages = (as_i32(t, dev) for t in (cached_lens, new_lens, free_pages))
-    table = torch.empty((nseq, max_pages), dtype=torch.int32, device=dev)
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    ints = torch.empty(3 * nseq + 4, dtype=torch.int32, device=dev)
-    cu_q, cu_k = ints[:nseq + 1], ints[nseq + 1:2 * nseq + 2]
-    lens, pages = ints[2 * nseq + 2:3 * nseq + 2], ints[3 * nseq + 2:]
+    table = cached_lens.new_empty((nseq, max_pages))
+    slots = cached_lens.new_empty(num_tokens, dtype=torch.int64)
+    cu_q, cu_k, lens, pages = cached_lens.new_empty(3 * nseq + 4).split((nseq + 1, nseq + 1, nseq, 2))
     with _lib.on_device(dev):
         _lib.check(_lib.load().fa4cp_paged_block_tables(
             cached_lens.data_ptr(), new_lens.data_ptr(), nseq, free_pages.data_ptr(),
@@ -124,7 +122,7 @@ def paged_tree_mask(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, *,
     assert parents.dim() == 1 and cu_seqlens_q.dim() == 1, "parents is [T], cu_seqlens_q [nseq + 1]"
     parents, cu = as_i32(parents, dev), as_i32(cu_seqlens_q, dev)
     total = parents.shape[0]
-    mask = torch.empty((total, (max_nodes + 63) // 64), dtype=torch.int64, device=dev)
+    mask = parents.new_empty((total, (max_nodes + 63) // 64), dtype=torch.int64)
     with _lib.on_device(dev):
         _lib.check(_lib.load().fa4cp_paged_tree_mask(
             parents.data_ptr(), cu.data_ptr(), cu.numel() - 1, total, max_nodes, mask.data_ptr(),
@@ -144,8 +142,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     ``e4m3(clamp(x / descale))`` with the descales (scalar, ``[H_kv]`` or ``(1, H_kv)``) that
     the attention multiplies back (``None``: 1).  Tokens with a slot outside the pools (-1)
     are skipped.  Slots must differ: two tokens with one slot leave a mixture of their rows."""
-    _check_pools(k_pages, v_pages)
-    _lib.require_cuda(k, v, slot_mapping)
+    _check_pools(k_pages, v_pages, k, v, slot_mapping)
     num_pages, page_size, h_kv, d = k_pages.shape
     assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype, "k and v are [T, H_kv, D]"
     assert k.shape[1:] == (h_kv, d), "the rows and the pools differ in H_kv or D"
@@ -158,7 +155,9 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     kd, vd = norm_descale(k_descale, h_kv, dev), norm_descale(v_descale, h_kv, dev)
     ks, vs = pool_strides(k_pages, "k_pages"), pool_strides(v_pages, "v_pages")
     k, v = rows16(k), rows16(v)
-    slots = slot_mapping.to(torch.int64).contiguous()
+    slots = slot_mapping
+    if slots.dtype is not torch.int64 or not slots.is_contiguous():
+        slots = slots.to(torch.int64).contiguous()
     with _lib.on_device(dev):
         _lib.check(_lib.load().fa4cp_paged_kv_write(
             k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k_pages.data_ptr(),
@@ -181,8 +180,7 @@ def paged_kv_accept(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     path ascend, since parents come before children).  Row ``cached + i`` becomes what row
     ``cached + accepted[j, i]`` was; the rows behind the path keep what they hold.  Rows
     without a valid page are skipped."""
-    _check_pools(k_pages, v_pages)
-    _lib.require_cuda(block_table, cached_lens, accepted)
+    _check_pools(k_pages, v_pages, block_table, cached_lens, accepted)
     num_pages, page_size, h_kv, d = k_pages.shape
     dev = k_pages.device
     nseq = cached_lens.shape[0]
@@ -192,7 +190,7 @@ def paged_kv_accept(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     assert cu_seqlens_q.numel() == nseq + 1, "cu_seqlens_q is [nseq + 1]"
     ks, vs = pool_strides(k_pages, "k_pages"), pool_strides(v_pages, "v_pages")
     bt, cached, acc, cu = (as_i32(t, dev) for t in (block_table, cached_lens, accepted, cu_seqlens_q))
-    lens = torch.empty(nseq, dtype=torch.int32, device=dev)
+    lens = cached.new_empty(nseq)
     with _lib.on_device(dev):
         _lib.check(_lib.load().fa4cp_paged_kv_accept(
             k_pages.data_ptr(), v_pages.data_ptr(), ks, vs, num_pages, page_size, bt.data_ptr(),
