@@ -65,9 +65,6 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: P <= 256
 constexpr int BM = 128;
-// An e4m3 V is attended as f16 values x this factor: 448 x 146 is the largest product that f16
-// holds, 480 x 146 (what NaN's bits would stand for) overflows
-constexpr float kV8Scale = 146.f;
 
 // codes written to the device status word when a bounded wait gives up
 enum : int {
@@ -123,14 +120,15 @@ struct TreeTraits {
   static constexpr int OFF_RAW = OFF_V + VS * V_BYTES;
   static constexpr int OFF_ROWS = OFF_RAW + RS * RAW_BYTES;
   // per row: running maximum [BM]; per item parity and warpgroup: maximum, sum, flag [2][2][BM]
-  static constexpr int OFF_ITEMS = OFF_ROWS + BM * 4 + 4 * BM * 12;
+  static constexpr int NWG = 2, W0 = 4 * NWG;  // softmax warpgroups, and the first warp behind them
+  static constexpr int OFF_ITEMS = OFF_ROWS + BM * 4 + 2 * NWG * BM * 12;
   static constexpr int OFF_BAR = OFF_ITEMS + kItems * 48;
   // k_full, k_empty [KS]; v_full, v_empty [VS]; r_full, r_empty [RS]; s_full, p_full, o_done
-  // [NB]; max_known[8] (warpgroup, warp), v_fixed[2], q_full, o_free, joined, teardown;
+  // [NB]; max_known[W0] (warpgroup, warp), v_fixed[NWG], q_full, o_free, joined, teardown;
   // q_staged, item_full, item_free [kItems]
   static constexpr bool APART = D <= 128;
   static constexpr int NB = D == 128 ? 3 : 4;  // S buffers: what TMEM leaves
-  static constexpr int NUM_BARS = 2 * (KS + VS + RS) + 3 * NB + 14 + 3 * kItems;
+  static constexpr int NUM_BARS = 2 * (KS + VS + RS) + 3 * NB + 5 * NWG + 4 + 3 * kItems;
   // q_staged(i) is waited for before q_staged(i + kItems) can complete: the items between them
   // take two slots of the K ring each, so the latter needs the former's slots back
   static_assert(KS < 2 * kItems, "Q staging ring");
@@ -138,13 +136,13 @@ struct TreeTraits {
   static constexpr int SMEM_BYTES = OFF_MISC + 128 + 1024;
   // an e4m3 V tile is widened by one warp (two at head_dim 256), the next tile by the next
   static constexpr int CONV_WARPS = KV8 ? 4 : 0, CONV_TEAM = D == 256 ? 2 : 1;
-  static constexpr int THREADS = 384 + CONV_WARPS * 32;
+  static constexpr int THREADS = W0 * 32 + 128 + CONV_WARPS * 32;
   // setmaxnreg split, in registers a thread of a warpgroup; the launch gives 512 x 128 or
   // 384 x 168 registers
   static constexpr int REGS_SOFTMAX = KV8 ? 168 : 184, REGS_CONTROL = KV8 ? 80 : 136, REGS_CONV = 96;
-  static_assert(128 * (2 * REGS_SOFTMAX + REGS_CONTROL) + 32 * CONV_WARPS * REGS_CONV <=
-                    (KV8 ? 512 * 128 : 384 * 168), "register split exceeds the launch allocation");
-  static constexpr int TM_S = 0, TM_O = NB * BN, TM_Q = TM_O + (APART ? 2 : 1) * D;
+  static_assert(128 * (NWG * REGS_SOFTMAX + REGS_CONTROL) + 32 * CONV_WARPS * REGS_CONV <=
+                    THREADS * (65536 / THREADS / 8 * 8), "register split exceeds the launch allocation");
+  static constexpr int TM_S = 0, TM_O = NB * BN, TM_Q = TM_O + (APART ? NWG : 1) * D;
   static_assert(TM_Q + D / 2 <= 512, "TMEM budget");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
 };
@@ -157,42 +155,18 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int 
       "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
       : "memory");
 }
-// mbar_wait with the non-suspending test: the hand-overs between this kernel's roles are short,
-// and waking from a suspended wait costs more than they take.
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort, int code, int* status) {
-  if (mbar_test(bar, parity)) return true;
-  const long long t0 = clock64();
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_test(bar, parity)) return true;
-    if ((it & 1023u) == 0) {
-      if (*abort) return false;
-      if (*reinterpret_cast<volatile int*>(status) != 0) {  // another CTA already gave up
-        *abort = 1;
-        return false;
-      }
-      if (clock64() - t0 > kWaitLimitCycles) {
-        *abort = 1;
-        atomicCAS(status, 0, code);
-        return false;
-      }
-    }
-  }
-}
 // As make_desc_sw128 with the 64-byte swizzle (mode 4).
 __device__ __forceinline__ uint64_t make_desc_sw64(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
   return (make_desc_sw128(saddr, lbo_bytes, sbo_bytes) & ~(7ull << 61)) | (4ull << 61);
 }
+// A ring's current slot and the parity of its fill.
+template <int N>
+struct Ring {
+  uint32_t slot = 0, parity = 0;
+  __device__ __forceinline__ void step() {
+    if (++slot == uint32_t(N)) { slot = 0; parity ^= 1; }
+  }
+};
 // One lane of a converged warp, chosen by the hardware: code under it stays warp-uniform for the
 // compiler, so descriptors and addresses live in uniform registers.
 __device__ __forceinline__ bool elect_one() {
@@ -413,10 +387,10 @@ __device__ __forceinline__ void q16_terms(const uint4 a, const uint4 b, float f,
 
 // Rows that see a key whose V row is not finite, after the finite part has been written to
 // their row of the result (16-bit) or of a partial (fp32): the non-finite values themselves are
-// added (their weight is positive), columns [d0, d0 + D / 2).  Rare; reads V again from the pool.
-template <int D>
+// added (their weight is positive): of every STEP blocks of 16 columns the one at `first`.  Rare; reads V again from the pool.
+template <int D, int STEP>
 __device__ __forceinline__ void add_nonfinite(const TreeParams& p, int seq, int kvh, int ctx, int lim,
-                                              int64_t tok, int node, int key0, int key1, int d0,
+                                              int64_t tok, int node, int key0, int key1, int first,
                                               uint16_t* out_row, float* part_row) {
 #pragma unroll 1
   for (int key = max(max(key0, ctx), 0); key < min(key1, lim); ++key) {
@@ -426,7 +400,7 @@ __device__ __forceinline__ void add_nonfinite(const TreeParams& p, int seq, int 
     if (page < 0 || page >= p.num_pages) continue;
     const uint8_t* row = p.v + page * p.v_page + (key - e * p.page_size) * p.v_row + kvh * p.v_head;
 #pragma unroll 1
-    for (int d = d0; d < d0 + D / 2; ++d) {
+    for (int d = first * 16; d < D; d += (d & 15) == 15 ? (STEP - 1) * 16 + 1 : 1) {
       float x;
       if (p.kv_dtype == FA4CP_DTYPE_E4M3) {
         if ((row[d] & 0x7F) != 0x7F) continue;
@@ -451,7 +425,7 @@ template <class TR>
 __global__ void __launch_bounds__(TR::THREADS, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                      const TreeParams p) {
-  constexpr int D = TR::D, BN = TR::BN;
+  constexpr int D = TR::D, BN = TR::BN, NWG = TR::NWG, W0 = TR::W0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -474,22 +448,23 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
   auto p_full = [&](uint32_t i) { return BAR(B1 + NB + int(i % NB)); };
   auto o_done = [&](uint32_t i) { return BAR(B1 + 2 * NB + int(i % NB)); };
   auto max_known = [&](int wg, int w4) { return BAR(B2 + wg * 4 + w4); };
-  auto v_fixed = [&](int wg) { return BAR(B2 + 8 + wg); };
-  const uint32_t q_full = BAR(B2 + 10), o_free = BAR(B2 + 11), joined = BAR(B2 + 12), td_bar = BAR(B2 + 13);
-  auto q_staged = [&](int i) { return BAR(B2 + 14 + i % kItems); };
-  auto item_full = [&](int i) { return BAR(B2 + 14 + kItems + i % kItems); };
-  auto item_free = [&](int i) { return BAR(B2 + 14 + 2 * kItems + i % kItems); };
+  auto v_fixed = [&](int wg) { return BAR(B2 + W0 + wg); };
+  constexpr int B3 = B2 + 5 * NWG, B4 = B3 + 4;
+  const uint32_t q_full = BAR(B3), o_free = BAR(B3 + 1), joined = BAR(B3 + 2), td_bar = BAR(B3 + 3);
+  auto q_staged = [&](int i) { return BAR(B4 + i % kItems); };
+  auto item_full = [&](int i) { return BAR(B4 + kItems + i % kItems); };
+  auto item_free = [&](int i) { return BAR(B4 + 2 * kItems + i % kItems); };
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + TR::OFF_MISC);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  volatile uint32_t* bad = tmem_slot + 4;  // [2 warpgroups][2][4]: keys with a non-finite V row
+  volatile uint32_t* bad = tmem_slot + 4;  // [warpgroups][2][4]: keys with a non-finite V row
   volatile float* row_max = reinterpret_cast<volatile float*>(smem + TR::OFF_ROWS);
-  volatile float* end_max = row_max + BM;                // [2 items][2 warpgroups][BM]
-  volatile float* end_sum = end_max + 4 * BM;
-  volatile int* end_bad = reinterpret_cast<volatile int*>(end_sum + 4 * BM);
+  volatile float* end_max = row_max + BM;                // [2 items][warpgroups][BM]
+  volatile float* end_sum = end_max + 2 * NWG * BM;
+  volatile int* end_bad = reinterpret_cast<volatile int*>(end_sum + 2 * NWG * BM);
   Item* items = reinterpret_cast<Item*>(smem + TR::OFF_ITEMS);
   int* status = &g_tree_status;
 
-  if (threadIdx.x == 32 * 8) {
+  if (threadIdx.x == 32 * W0) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
     for (int s = 0; s < TR::KS; ++s) {
@@ -509,23 +484,22 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       mbar_init(p_full(b), 4);
       mbar_init(o_done(b), 1);
     }
-    mbar_init(v_fixed(0), 4);
-    mbar_init(v_fixed(1), 4);
-    for (int i = 0; i < 8; ++i) mbar_init(max_known(0, i), 1);
-    mbar_init(q_full, 8);
-    mbar_init(o_free, 8);
-    mbar_init(joined, 8);
+    for (int g = 0; g < NWG; ++g) mbar_init(v_fixed(g), 4);
+    for (int i = 0; i < W0; ++i) mbar_init(max_known(0, i), 1);
+    mbar_init(q_full, W0);
+    mbar_init(o_free, W0);
+    mbar_init(joined, W0);
     mbar_init(td_bar, 2);
     for (int i = 0; i < kItems; ++i) {
       mbar_init(q_staged(i), 32);
       mbar_init(item_full(i), 1);
-      mbar_init(item_free(i), 11 + TR::CONV_WARPS);  // softmax 8, V, S, PV, converters
+      mbar_init(item_free(i), W0 + 3 + TR::CONV_WARPS);  // softmax, V, S, PV, converters
     }
     *abort = 0;
     fence_mbar_init();
   }
   if (threadIdx.x == 0) p.desc[2 * cta] = make_int4(0, 0, 0, 0);  // this thread names a split row tile later
-  if (warp == 9) {
+  if (warp == W0 + 1) {
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
@@ -548,19 +522,17 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
 
   if (share.t0 >= share.t1) {
     // no work (uniform for the CTA): on to the release of TMEM
-  } else if (warp >= 12) {
+  } else if (warp >= W0 + 4) {
     if constexpr (TR::KV8) {
       // ---------------------------------------------------------- V: e4m3 -> f16
-      // Bits s eeee mmm moved to f16's places are the value x 2^-8, subnormals included; one
-      // product makes it x kV8Scale, exactly (4 x 7 significant bits), and e4m3's NaN, which
-      // the bits take for 480, infinite.  (The conversion instruction runs at a quarter of the
-      // rate, on the unit that the softmax's exponentials need.)  Each 16-byte piece becomes
-      // two pieces of the swizzled operand tile.  Eight lanes take the 64-byte halves of two
-      // rows crosswise (row r from chunk a, row r + 1 from chunk a ^ 1), so neither the reads
-      // nor the writes meet in a bank.
+      // Each 16-byte piece becomes two pieces of the swizzled operand tile.  (Moving the bits with
+      // integer instructions instead takes three times as many of them: 423 us against 388, e4m3,
+      // head_dim 128, 32 requests of 64 tokens and up to 16K cached.)  Eight lanes take the 64-byte
+      // halves of two rows crosswise (row r from chunk a, row r + 1 from chunk a ^ 1), so neither
+      // the reads nor the writes meet in a bank.
       setmaxnreg_dec<TR::REGS_CONV>();
       constexpr int TEAM = TR::CONV_TEAM, TEAMS = 4 / TEAM;
-      const int team = (warp - 12) / TEAM, t = (warp - 12) % TEAM * 32 + lane;
+      const int team = (warp - W0 - 4) / TEAM, t = (warp - W0 - 4) % TEAM * 32 + lane;
       const int half = (t & 7) >> 2, piece = t & 3, unit = t >> 3;
       const int row0 = unit / TR::V_COLS * 2 + half, a = unit % TR::V_COLS;
       const int ch = TR::V_COLS > 1 && half ? a ^ 1 : a;
@@ -568,16 +540,14 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       uint8_t* dst0 = smem + TR::OFF_V + ch * TR::V_CHUNK + row0 * 128;
       constexpr int PIECES = BN * D / 16 / (32 * TEAM);  // 16-byte pieces a thread
       constexpr int STEP = 8 * TEAM / TR::V_COLS;        // rows from one to the next
-      const __half2 k146 = __floats2half2_rn(kV8Scale * 256.f, kV8Scale * 256.f);
       uint32_t i = 0;
       Item x;
       for (int item = 0; get_item(item, x); ++item) {
         bool ok = true;
         for (int j = 0; j < x.nt; ++j, ++i) {
           if (int(i % TEAMS) != team) continue;
-          ok = mbar_wait(r_full(i), phase(i, NR), abort, kErrRawFull, status);
-          if (ok && i >= uint32_t(TR::VS))
-            ok = mbar_wait(v_empty(i), phase(i, TR::VS) ^ 1, abort, kErrVEmpty, status);
+          ok = mbar_wait(r_full(i), phase(i, NR), abort, kErrRawFull, status) &&
+               mbar_wait(v_empty(i), phase(i, TR::VS) ^ 1, abort, kErrVEmpty, status);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           const uint8_t* src = src0 + (i % NR) * TR::RAW_BYTES;
@@ -592,17 +562,11 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
               const uint32_t w[4] = {in[u].x, in[u].y, in[u].z, in[u].w};
               uint32_t o[8];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                // bytes b3 b2 b1 b0 -> halfwords (b1, b0) and (b3, b2)
-                const uint32_t lo = __byte_perm(w[k], 0u, 0x1404), hi = __byte_perm(w[k], 0u, 0x3424);
-                o[2 * k] = (lo & 0x80008000u) | ((lo >> 1) & 0x3F803F80u);
-                o[2 * k + 1] = (hi & 0x80008000u) | ((hi >> 1) & 0x3F803F80u);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&o[2 * k + h]), k146);
-                  o[2 * k + h] = *reinterpret_cast<const uint32_t*>(&v);
-                }
-              }
+              for (int k = 0; k < 4; ++k)
+                asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+                    "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+                    : "=r"(o[2 * k]), "=r"(o[2 * k + 1])
+                    : "r"(w[k]));
               const int row = row0 + (u0 + u) * STEP;
               uint8_t* to = dst + (u0 + u) * STEP * 128;
               const int at = ((2 * piece) ^ (row & 7)) * 16;
@@ -620,12 +584,12 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         if (!ok) break;
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= W0) {
     setmaxnreg_dec<TR::REGS_CONTROL>();
-    if (warp == 8 || warp == 10) {
+    if (warp == W0 || warp == W0 + 2) {
       // ---------------------------------------------------------- producers
       // a lane copies one (page piece, swizzled column) of a tile
-      const bool is_v = warp == 10;
+      const bool is_v = warp == W0 + 2;
       const int slots = is_v ? (TR::KV8 ? TR::RS : TR::VS) : TR::KS;
       const int bytes = is_v ? (TR::KV8 ? TR::RAW_BYTES : TR::V_BYTES) : TR::K_BYTES;
       const int cols = is_v ? (TR::KV8 ? 1 : TR::V_COLS) : TR::K_COLS;
@@ -748,28 +712,43 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       // uniform registers (issuing from one lane's own branch took 1.3 times as long).
       const int fmt = p.kv_dtype == FA4CP_DTYPE_BF16 ? 1 : 0;  // (e4m3 is format 0, and V is f16)
       const uint32_t ring = smem_u32(smem);
-      uint32_t it = 0;
+      // The loop is what a tile takes here (about 900 cycles when it divided its ring indices), so
+      // slots and parities are carried along.  A tile waits for two barriers: one after the other,
+      // or, at head_dim 64, by a lane each (e4m3, 64 tokens and one: 282 and 145 us against 300 and
+      // 152; at head_dim 128 385 and 175 against 346 and 153).
+      auto wait_two = [&](uint32_t bar_a, uint32_t par_a, int code_a, uint32_t bar_b, uint32_t par_b, int code_b) -> bool {
+        bool ok;
+        if constexpr (D == 64) {
+          const bool a = lane == 0;
+          ok = mbar_wait(a ? bar_a : bar_b, a ? par_a : par_b, abort, a ? code_a : code_b, status);
+        } else {
+          ok = mbar_wait(bar_a, par_a, abort, code_a, status) && mbar_wait(bar_b, par_b, abort, code_b, status);
+        }
+        return __all_sync(0xffffffffu, ok);
+      };
       Item x;
-      if (warp == 9) {
+      if (warp == W0 + 1) {
         const uint32_t idesc = make_idesc(BM, BN, fmt, fmt, 0, 0);
         const int q_terms = TR::KV8 && p.q_dtype != FA4CP_DTYPE_E4M3 ? 2 : 1;
         // 32 bytes along D a step, then the next swizzled column
         constexpr int STEPS = D * TR::KEL / 32, PER_COL = TR::K_SWZ / 32;
+        const uint64_t desc0 = TR::K_SWZ == 128 ? make_desc_sw128(ring, 16, 1024) : make_desc_sw64(ring, 16, 512);
+        const uint32_t a = tmem + uint32_t(TR::TM_Q);
+        Ring<TR::KS> k;
+        Ring<NB> sb;
         for (int item = 0; get_item(item, x); ++item) {
           bool ok = __all_sync(0xffffffffu, mbar_wait(q_full, uint32_t(item) & 1, abort, kErrQFull, status));
           if (!ok) break;
           if (lane < x.q_slots) mbar_arrive(k_empty(x.k_idx + lane));  // Q has been read
-          uint32_t ki = x.k_idx + x.q_slots;
-          for (int j = 0; j < x.nt; ++j, ++it, ++ki) {
-            if (it >= uint32_t(NB))  // the P over the buffer's last S has been multiplied
-              ok = mbar_wait(o_done(it - NB), phase(it - NB, NB), abort, kErrSFree, status);
-            if (ok) ok = mbar_wait(k_full(ki), phase(ki, TR::KS), abort, kErrKFull, status);
-            ok = __all_sync(0xffffffffu, ok);
+          for (int i = 0; i < x.q_slots; ++i) k.step();
+          for (int j = 0; j < x.nt; ++j) {
+            // the P over the buffer's last S has been multiplied (a buffer's first use waits for a
+            // phase that counts as complete), and the K tile is there
+            ok = wait_two(BAR(B1 + 2 * NB + int(sb.slot)), sb.parity ^ 1, kErrSFree, BAR(int(k.slot)), k.parity, kErrKFull);
             if (!ok) break;
             tc_fence_after();
-            const uint32_t sK = ring + (ki % TR::KS) * TR::K_BYTES;
-            const uint64_t desc = TR::K_SWZ == 128 ? make_desc_sw128(sK, 16, 1024) : make_desc_sw64(sK, 16, 512);
-            const uint32_t d = tmem + uint32_t(TR::TM_S) + it % NB * BN, a = tmem + uint32_t(TR::TM_Q);
+            const uint64_t desc = desc0 + uint64_t(k.slot * uint32_t(TR::K_BYTES / 16));
+            const uint32_t d = tmem + uint32_t(TR::TM_S) + sb.slot * BN;
             if (elect_one()) {
               if constexpr (TR::KV8) {
 #pragma unroll
@@ -788,34 +767,43 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
                   mma_f16_ts(d, a + uint32_t(kk * 8), desc + uint64_t((kk / PER_COL * BN * TR::K_SWZ + kk % PER_COL * 32) / 16),
                              idesc, kk > 0 ? 1u : 0u);
               }
-              tc_commit(s_full(it));
-              tc_commit(k_empty(ki));
+              tc_commit(BAR(B1 + int(sb.slot)));
+              tc_commit(BAR(TR::KS + int(k.slot)));
             }
             __syncwarp();
+            k.step();
+            sb.step();
           }
           if (!ok) break;
         }
       } else {
         const uint32_t idesc = make_idesc(BM, D, fmt, fmt, 0, 1);
+        const uint64_t desc0 = make_desc_sw128(ring + TR::OFF_V, TR::V_CHUNK, 1024);
+        Ring<TR::VS> v;
+        Ring<NB> sb;
+        Ring<TR::APART ? NWG : 1> ob;
         for (int item = 0; get_item(item, x); ++item) {
           bool ok = true;
-          for (int j = 0; j < x.nt; ++j, ++it) {
-            if (j == 0 && item > 0) ok = mbar_wait(o_free, uint32_t(item - 1) & 1, abort, kErrOFree, status);
-            if (ok) ok = mbar_wait(v_full(it), phase(it, TR::VS), abort, kErrVFull, status);
-            if (ok) ok = mbar_wait(p_full(it), phase(it, NB), abort, kErrPFull, status);
-            ok = __all_sync(0xffffffffu, ok);
+          if (item > 0)
+            ok = __all_sync(0xffffffffu, mbar_wait(o_free, uint32_t(item - 1) & 1, abort, kErrOFree, status));
+          for (int j = 0; ok && j < x.nt; ++j) {
+            ok = wait_two(BAR(2 * TR::KS + int(v.slot)), v.parity, kErrVFull, BAR(B1 + NB + int(sb.slot)), sb.parity, kErrPFull);
             if (!ok) break;
             tc_fence_after();
-            const uint64_t desc = make_desc_sw128(ring + TR::OFF_V + (it % TR::VS) * TR::V_BYTES, TR::V_CHUNK, 1024);
+            const uint64_t desc = desc0 + uint64_t(v.slot * uint32_t(TR::V_BYTES / 16));
+            const uint32_t o = tmem + uint32_t(TR::TM_O) + ob.slot * D, a = tmem + uint32_t(TR::TM_S) + sb.slot * BN;
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)  // 16 keys: 16 rows of 128 bytes further
-                mma_f16_ts(tmem + TR::TM_O + (TR::APART ? (it & 1) * D : 0u), tmem + uint32_t(TR::TM_S + kk * 8) + it % NB * BN,
-                           desc + uint64_t(kk * 16 * 128 / 16), idesc, (j > (TR::APART ? 1 : 0) || kk > 0) ? 1u : 0u);
-              tc_commit(o_done(it));
-              tc_commit(v_empty(it));
+                mma_f16_ts(o, a + uint32_t(kk * 8), desc + uint64_t(kk * 16 * 128 / 16), idesc,
+                           (j >= (TR::APART ? NWG : 1) || kk > 0) ? 1u : 0u);
+              tc_commit(BAR(B1 + 2 * NB + int(sb.slot)));
+              tc_commit(BAR(2 * TR::KS + TR::VS + int(v.slot)));
             }
             __syncwarp();
+            v.step();
+            sb.step();
+            ob.step();
           }
           if (!ok) break;
         }
@@ -879,7 +867,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           }
         }
 #pragma unroll 1
-        for (int c = wg * (D / 64); c < (wg + 1) * (D / 64); ++c) {  // 32 elements
+        for (int c = wg; c < D / 32; c += NWG) {  // 32 elements
           if constexpr (TR::KV8) {
             uint32_t hi[8], lo[8];
             if (q8) {
@@ -935,7 +923,6 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         if (p.q_descale) scale *= p.q_descale[x.kvh];
         if (p.k_descale) scale *= p.k_descale[x.kvh];
         if (p.v_descale) vscale = p.v_descale[x.kvh];
-        vscale *= 1.f / kV8Scale;
         // qf carries the sign of the descales, so the scale is positive; never 0, so that a
         // masked score stays -inf
         scale /= qf;
@@ -944,7 +931,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       // m: the maximum that this warpgroup's sum l (and its O) are relative to
       float m = kNegInf, l = 0.f;
       bool sees_bad = false;
-      for (int j = (it0 & 1) == uint32_t(wg) ? 0 : 1; j < n; j += 2) {
+      for (int j = int((uint32_t(wg) + NWG - it0 % NWG) % NWG); j < n; j += NWG) {
         const uint32_t it = it0 + j;
         ok = mbar_wait(s_full(it), phase(it, NB), abort, kErrSFull, status);
         if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
@@ -958,7 +945,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         for (int c = 0; c < C; ++c) vis[c] = 0u;
         // the tile before has settled the maximum (the other warpgroup's tile)
         auto max_settled = [&]() -> bool {
-          return it == 0 || __all_sync(0xffffffffu, mbar_wait(max_known(wg ^ 1, w4), ((it - 1) >> 1) & 1, abort,
+          return it == 0 || __all_sync(0xffffffffu, mbar_wait(max_known((wg + NWG - 1) % NWG, w4), phase(it - 1, NWG), abort,
                                                               kErrMax, status));
         };
         if (active) {
@@ -1006,7 +993,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
             if (m != kNegInf) l *= ex2_approx((m - m_new) * scale);
             m = m_new;
           }
-          constexpr int MINE = TR::APART ? 2 : 1;  // PV(it - MINE) was the last one into this O
+          constexpr int MINE = TR::APART ? NWG : 1;  // PV(it - MINE) was the last one into this O
           if (j >= MINE && __any_sync(0xffffffffu, raise)) {
             const float f = !raise ? 1.f : so_far == kNegInf ? 0.f : ex2_approx((so_far - m_new) * scale);
             ok = mbar_wait(o_done(it - MINE), phase(it - MINE, NB), abort, kErrODone, status);
@@ -1092,9 +1079,9 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       }
       if (aborted) break;
 
-      // what the other warpgroup needs to finish the row
+      // what the other warpgroups need to finish the row
       const uint32_t last = it0 + n - 1;
-      const int set = (item & 1) * 2;
+      const int set = (item & 1) * NWG;
       end_max[(set + wg) * BM + t] = m;
       end_sum[(set + wg) * BM + t] = l;
       end_bad[(set + wg) * BM + t] = sees_bad;
@@ -1114,19 +1101,22 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       // Apart: O = f0 O0 + f1 O1.  Shared: O is relative to the last tile's maximum.
-      float part_max[2], part_f[2];
+      float part_f[NWG];
 #pragma unroll
-      for (int g = 0; g < 2; ++g) part_max[g] = end_max[(set + g) * BM + t];
-      m = TR::APART ? fmaxf(part_max[0], part_max[1]) : part_max[last & 1];
+      for (int g = 0; g < NWG; ++g) part_f[g] = end_max[(set + g) * BM + t];
+      m = end_max[(set + last % NWG) * BM + t];
+      if (TR::APART) {
+#pragma unroll
+        for (int g = 0; g < NWG; ++g) m = fmaxf(m, part_f[g]);
+      }
       l = 0.f;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const float lg = end_sum[(set + g) * BM + t];
-        part_f[g] = part_max[g] == m ? 1.f : part_max[g] == kNegInf ? 0.f : ex2_approx((part_max[g] - m) * scale);
-        l += part_max[g] == kNegInf ? lg : lg * part_f[g];  // (NaN sums have no maximum)
+      for (int g = 0; g < NWG; ++g) {
+        const float lg = end_sum[(set + g) * BM + t], mg = part_f[g];
+        part_f[g] = mg == m ? 1.f : mg == kNegInf ? 0.f : ex2_approx((mg - m) * scale);
+        l += mg == kNegInf ? lg : lg * part_f[g];  // (NaN sums have no maximum)
         sees_bad |= end_bad[(set + g) * BM + t] != 0;
       }
-      const bool two = TR::APART && n > 1;  // the last tile's O, and the other one
       const bool whole = n == x.kt;
       const int part = 2 * cta + (x.kt0 == 0 ? 1 : 0);
       const float mult = whole ? (l == 0.f ? 0.f : vscale / l) : vscale;
@@ -1134,26 +1124,30 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       float* prow = p.part_o + (int64_t(part) * BM + t) * D;
       if (active) {
 #pragma unroll 1
-        for (int c = wg * (D / 32); c < (wg + 1) * (D / 32); ++c) {
-          uint32_t o[16], o2[16];
-          const uint32_t from = t_lane + uint32_t(TR::TM_O + c * 16);
-          tmem_ld16(from + (TR::APART ? (last & 1) * D : 0u), o);
-          if (two) tmem_ld16(from + (~last & 1) * D, o2);
-          tmem_wait_ld();
-          reg_fence16(o);
-          reg_fence16(o2);
+        for (int c = wg; c < D / 16; c += NWG) {
+          uint32_t o[16];
           float f[16];
+          const uint32_t from = t_lane + uint32_t(TR::TM_O + c * 16);
+          tmem_ld16(from, o);
+          if constexpr (TR::APART) {
+            uint32_t o1[16];
+            tmem_ld16(from + D, o1);
+            tmem_wait_ld();
+            reg_fence16(o);
+            reg_fence16(o1);
+            // a warpgroup without a tile of the item left an older item's O
+            const bool h0 = n > 1 || last % NWG == 0, h1 = n > 1 || last % NWG == 1;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            if (TR::APART) {
-              float y = __uint_as_float(o[e]) * part_f[last & 1];
-              if (two) y = fmaf(__uint_as_float(o2[e]), part_f[~last & 1], y);
-              o[e] = __float_as_uint(y);
+            for (int e = 0; e < 16; ++e) {
+              const float y = h0 ? __uint_as_float(o[e]) * part_f[0] : 0.f;
+              o[e] = __float_as_uint(h1 ? fmaf(__uint_as_float(o1[e]), part_f[1], y) : y);
             }
-            f[e] = __uint_as_float(o[e]) * mult;
-            // e4m3 has no infinities: one in O stands for a NaN of V
-            if (TR::KV8 && (o[e] & 0x7FFFFFFFu) == 0x7F800000u) f[e] = __uint_as_float(0x7FC00000u);
+          } else {
+            tmem_wait_ld();
+            reg_fence16(o);
           }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * mult;
           if (!valid) continue;
           if (whole) {
             uint32_t h[8];
@@ -1178,8 +1172,8 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           else __stcg(&p.part_ml[part * BM + t], make_float2(ms, l));
         }
         if (sees_bad)
-          add_nonfinite<D>(p, x.seq, x.kvh, ctx, x.lim, tok, node, x.kt0 * BN, (x.kt0 + n) * BN, wg * (D / 2),
-                           out_row, whole ? nullptr : prow);
+          add_nonfinite<D, NWG>(p, x.seq, x.kvh, ctx, x.lim, tok, node, x.kt0 * BN, (x.kt0 + n) * BN, wg, out_row,
+                                whole ? nullptr : prow);
       }
       if (threadIdx.x == 0 && !more && x.kt0 == 0 && !whole) {
         // the share's last item began here and goes on: this CTA's descriptor names it, and the
@@ -1196,7 +1190,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == W0 + 1) tmem_dealloc(tmem, 512);
 }
 
 // ---------------------------------------------------------------------------
@@ -1300,7 +1294,9 @@ int make_pool_map(CUtensorMap* map, const void* base, int num_pages, int page_si
                          swizzle == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
                          : swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                          : CU_TENSOR_MAP_SWIZZLE_NONE,
-                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                         // 128: a page's rows of one head may be no longer, and the other heads' rows
+                         // between them are another CTA's (f16, head_dim 64: 250 us, 256 took 263)
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_last_error("cuTensorMapEncodeTiled (pool) failed (%d)", int(r));
     return FA4CP_ERR_CUDA;
