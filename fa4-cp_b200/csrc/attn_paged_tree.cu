@@ -217,8 +217,6 @@ struct Share {
   int64_t t0, t1;        // this CTA's part
   int64_t total, each;   // each = total / g, the first `rest` CTAs take one more
   int g, rest;
-  int64_t off;  // t0 relative to its request's first tile
-  int seq;
   __device__ __forceinline__ int64_t begin(int c) const { return c * each + min(c, rest); }
   __device__ __forceinline__ int owner(int64_t x) const {  // the CTA whose part holds tile x
     const int64_t big = rest * (each + 1);
@@ -226,18 +224,31 @@ struct Share {
   }
 };
 
+// a / b, which are mostly below 2^32 (a 64-bit division takes four times as long).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
+
+// Where a share begins: `off` counted tiles into a request.
+struct Start {
+  Request r;
+  int seq;
+  int64_t off;
+};
+
 // All threads of the CTA.  A thread sums a run of requests, a block scan gives its run's first
-// tile, and the thread whose run holds t0 finds the request.
-template <int BN>
-__device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, int64_t* ws,
-                                            int64_t* found) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = blockDim.x >> 5;
-  const int per = (p.nseq + int(blockDim.x) - 1) / int(blockDim.x);
+// tile, and the thread whose run holds t0 finds the request and leaves it in `found`.  (All this
+// is a small batch's latency: each wait for global memory takes 700 cycles or so.)
+template <int BN, int THREADS>
+__device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, int64_t* ws, Start* found) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.nseq + THREADS - 1) / THREADS;
   const int j0 = min(tid * per, p.nseq), j1 = min(j0 + per, p.nseq);
   int64_t sum = 0;
+  Request r{};
 #pragma unroll 1
   for (int j = j0; j < j1; ++j) {
-    const Request r = load_request<BN>(p, j);
+    r = load_request<BN>(p, j);
     sum += int64_t(p.Hkv * r.mt) * (r.kt + kItemCost);
   }
   int64_t inc = sum;
@@ -249,15 +260,16 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
   if (lane == 31) ws[warp] = inc;
   __syncthreads();
   int64_t before = 0, total = 0;
-#pragma unroll 1
-  for (int w = 0; w < nw; ++w) {
-    if (w < warp) before += ws[w];
-    total += ws[w];
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const int64_t x = ws[w];
+    if (w < warp) before += x;
+    total += x;
   }
   Share s;
   s.total = total;
   s.g = int(min(int64_t(G), total));  // no CTA has an empty share between others
-  s.each = s.g > 0 ? total / s.g : 0;
+  s.each = s.g > 0 ? quotient(total, s.g) : 0;
   s.rest = int(total - s.each * s.g);
   s.t0 = c < s.g ? s.begin(c) : total;
   s.t1 = c < s.g ? s.begin(c + 1) : total;
@@ -265,19 +277,18 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
   if (s.t0 < s.t1 && first <= s.t0 && s.t0 < first + sum) {
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
-      const Request r = load_request<BN>(p, j);
+      if (per > 1) r = load_request<BN>(p, j);
       const int64_t tiles = int64_t(p.Hkv * r.mt) * (r.kt + kItemCost);
       if (s.t0 < first + tiles) {
-        found[0] = j;
-        found[1] = s.t0 - first;
+        found->r = r;
+        found->seq = j;
+        found->off = s.t0 - first;
         break;
       }
       first += tiles;
     }
   }
   __syncthreads();
-  s.seq = int(found[0]);
-  s.off = found[1];
   return s;
 }
 
@@ -288,12 +299,12 @@ struct Walk {
   int64_t left;         // counted tiles left of the share, from the current position on
   int seq, kvh, mtile, at;  // position: `at` counted tiles into the row tile
   int kt0, nt;          // the key tiles of the current row tile that are this CTA's
-  __device__ __forceinline__ void start(const TreeParams& p, const Share& s) {
-    seq = s.seq;
+  __device__ __forceinline__ void start(const Start& f, const Share& s) {
+    seq = f.seq;
     left = s.t1 - s.t0;
-    r = load_request<BN>(p, seq);
-    const int64_t item = s.off / (r.kt + kItemCost);
-    at = int(s.off - item * (r.kt + kItemCost));
+    r = f.r;
+    const int64_t item = quotient(f.off, r.kt + kItemCost);
+    at = int(f.off - item * (r.kt + kItemCost));
     kvh = int(item) / r.mt;
     mtile = int(item) - kvh * r.mt;
   }
@@ -504,9 +515,11 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
     tmem_relinquish();
   }
   tc_fence_before();
-  // (two __syncthreads; the scratch lies where the rings will be, before any copy is in flight)
+  // (two __syncthreads; the scratch lies where the K ring will be: warp W0, which reads it last,
+  // fills the ring)
   int64_t* sched = reinterpret_cast<int64_t*>(smem);
-  const Share share = find_share<BN>(p, cta, int(gridDim.x), sched, sched + 32);
+  Start* found = reinterpret_cast<Start*>(sched + 32);
+  const Share share = find_share<BN, TR::THREADS>(p, cta, int(gridDim.x), sched, found);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
@@ -615,14 +628,25 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       Walk<BN> w;
       bool more = true;
       if (!is_v) {
-        w.start(p, share);
+        w.start(*found, share);
+        __syncwarp();
         more = w.next(p);
       }
       bool ok = true;
       for (int item = 0; ok; ++item) {
         Item x;
+        int row = 0, page = -1;
+        // the page and row of this lane's piece of tile kt; -1 (zeros) where the cache has ended
+        auto lookup = [&](int kt, int& row) -> int {
+          const int64_t key = int64_t(kt) * BN + piece * box;
+          if (!mine || key >= x.lim) { row = 0; return -1; }
+          const int e = int(key) / p.page_size;
+          row = int(key) - e * p.page_size;
+          return p.block_table[int64_t(x.seq) * p.max_pages + e];
+        };
         if (is_v) {
           if (!get_item(item, x)) break;
+          page = lookup(x.kt0, row);
         } else {
           // publish the item
           if (item >= kItems)
@@ -645,13 +669,14 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
             mbar_arrive(item_full(item));
           }
           if (!more) break;
+          page = lookup(x.kt0, row);  // (read while Q is fetched)
           // its Q rows: 16-byte pieces, swizzled by the row so that a thread a row reads them
           // without bank conflicts
           const int per_row = q_row / 16, rows_step = 32 / per_row;  // per_row: 4 .. 32
           const int per_slot = TR::K_BYTES / q_row;
           const int c = lane & (per_row - 1);
-          int row = lane / per_row;
-          const int packed = x.mtile * BM + row;
+          int q = lane / per_row;
+          const int packed = x.mtile * BM + q;
           int node = packed / p.group, g = packed - node * p.group;
           for (int s = 0; ok && s < x.q_slots; ++s) {
             ok = wait_slot();
@@ -659,10 +684,10 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
             const uint32_t dst = smem_u32(smem) + slot * uint32_t(TR::K_BYTES);
             const int end = min(rows, (s + 1) * per_slot);
 #pragma unroll 1
-            for (; row < end; row += rows_step) {
+            for (; q < end; q += rows_step) {
               const uint8_t* src = p.q + (int64_t(x.token0) + node) * p.q_stride +
                                    int64_t(x.kvh * p.group + g) * q_row + c * 16;
-              const uint32_t to = dst + uint32_t((row - s * per_slot) * q_row + ((c ^ (row & 7 & (per_row - 1))) * 16));
+              const uint32_t to = dst + uint32_t((q - s * per_slot) * q_row + ((c ^ (q & 7 & (per_row - 1))) * 16));
               asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
               g += rows_step;
               while (g >= p.group) { g -= p.group; ++node; }
@@ -673,15 +698,6 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           if (!ok) break;
           asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(q_staged(item)) : "memory");
         }
-        // the page and row of this lane's piece of tile kt; -1 (zeros) where the cache has ended
-        auto lookup = [&](int kt, int& row) -> int {
-          const int64_t key = int64_t(kt) * BN + piece * box;
-          if (!mine || key >= x.lim) { row = 0; return -1; }
-          const int e = int(key) / p.page_size;
-          row = int(key) - e * p.page_size;
-          return p.block_table[int64_t(x.seq) * p.max_pages + e];
-        };
-        int row, page = lookup(x.kt0, row);
         for (int j = 0; j < x.nt; ++j) {
           int nrow = 0, npage = -1;  // asked for before this tile waits for its slot
           if (j + 1 < x.nt) npage = lookup(x.kt0 + j + 1, nrow);
@@ -1202,6 +1218,10 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
 template <int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
   const int c = blockIdx.x, lane = threadIdx.x & 31;
+  // launched as the attention ends (0.3 to 0.7 us earlier than a plain launch, of 14 to 19 us for
+  // one request; letting it come as early as the attention begins cost 1 us): the parts are there
+  // from here on
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 d0 = p.desc[2 * c];
   if (d0.x == 0) return;
   const int4 d1 = p.desc[2 * c + 1];
@@ -1333,7 +1353,16 @@ int launch_tree(const void* k_pages, const void* v_pages, const int64_t* ks, con
   if (int rc = check_launch("attn_fwd_paged_tree")) return rc;
   const int64_t most = int64_t(max_seqlen_q) * p.group;  // rows of a row tile
   const int blocks = int(((most < BM ? most : BM) + 7) / 8);
-  tree_combine_kernel<TR::D><<<dim3(unsigned(grid), unsigned(blocks)), 256, 0, st>>>(p);
+  cudaLaunchAttribute overlap{};
+  overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  overlap.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(grid), unsigned(blocks));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cfg.attrs = &overlap;
+  cfg.numAttrs = 1;
+  FA4CP_CHECK_CUDA(cudaLaunchKernelEx(&cfg, tree_combine_kernel<TR::D>, p));
   return check_launch("attn_fwd_paged_tree (combine)");
 }
 
