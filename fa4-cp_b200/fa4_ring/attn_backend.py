@@ -260,8 +260,9 @@ def rows16(x: torch.Tensor) -> torch.Tensor:
     """``x [T, H, D]`` as rows of ``H * D`` dense elements at a 16-byte aligned token stride:
     a slice of a fused projection is taken as it is, anything else is copied."""
     _, heads, d = x.shape
-    if (x.stride(2) == 1 and (heads == 1 or x.stride(1) == d)
-            and x.stride(0) * x.element_size() % 16 == 0 and x.data_ptr() % 16 == 0):
+    token, head, elem = x.stride()
+    if (elem == 1 and (head == d or heads == 1)
+            and (token * x.element_size() | x.data_ptr()) & 15 == 0):
         return x
     return x.contiguous()
 
@@ -302,9 +303,9 @@ def b200_attn_paged_tree(
     word ``w`` is node ``64 w + m`` of its request.  Without a mask a token sees the new rows
     up to its own (bottom-right causal, as :func:`b200_attn`); one token a request is decode.
 
-    q is f16 / bf16 with K/V of its dtype, or f16 / bf16 / e4m3 with e4m3 K/V (and their
-    descales, scalar, ``[H_kv]`` or ``(1, H_kv)``); head_dim 64, 128 or 256; page_size 16, 32,
-    64 or a multiple of 128.  The pools may be views of another layout.  Long caches are split
+    q is f16 / bf16 with K/V of its dtype, or bf16 / e4m3 with e4m3 K/V (and their descales,
+    scalar, ``[H_kv]`` or ``(1, H_kv)``); head_dim 64, 128 or 256; page_size 16, 32, 64 or a
+    multiple of 128; ``max_seqlen_q`` bounds the requests' new tokens.  The pools may be views of another layout.  Long caches are split
     over the GPU whatever the batch.  Returns ``(out [T, H, D], lse [T, H] fp32 natural log)``;
     out has q's dtype (bf16 for e4m3).  A row that sees no key gets out 0, lse -inf.  What lies
     behind ``seq_lens`` in a page never reaches the result, nor does what a token does not see.
@@ -314,8 +315,8 @@ def b200_attn_paged_tree(
     assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, "pools are [pages, page, H_kv, D]"
     assert k_pages.dtype == v_pages.dtype, "the pools must share a dtype"
     num_pages, page_size, h_kv, D = k_pages.shape
-    T, H = q.shape[:2]
-    assert q.shape[2] == D and H % h_kv == 0, f"q [{T}, {H}, {q.shape[2]}] does not fit H_kv={h_kv}, D={D}"
+    T, H, dq = q.shape
+    assert dq == D and H % h_kv == 0, f"q [{T}, {H}, {dq}] does not fit H_kv={h_kv}, D={D}"
     dev = q.device
     assert k_pages.device == v_pages.device == dev, "q and the pools must be on one device"
     nseq = cu_seqlens_q.numel() - 1

@@ -95,7 +95,8 @@ def paged_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor,
     cached_lens, new_lens, free_pages = (as_i32(t, dev) for t in (cached_lens, new_lens, free_pages))
     table = cached_lens.new_empty((nseq, max_pages))
     slots = cached_lens.new_empty(num_tokens, dtype=torch.int64)
-    cu_q, cu_k, lens, pages = cached_lens.new_empty(3 * nseq + 4).split((nseq + 1, nseq + 1, nseq, 2))
+    cu_q, cu_k, lens, pages = cached_lens.new_empty(3 * nseq + 4).unsafe_split_with_sizes(
+        (nseq + 1, nseq + 1, nseq, 2))
     with _lib.on_device(dev):
         _lib.check(_lib.load().fa4cp_paged_block_tables(
             cached_lens.data_ptr(), new_lens.data_ptr(), nseq, free_pages.data_ptr(),
@@ -145,8 +146,9 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     _check_pools(k_pages, v_pages, k, v, slot_mapping)
     num_pages, page_size, h_kv, d = k_pages.shape
     assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype, "k and v are [T, H_kv, D]"
-    assert k.shape[1:] == (h_kv, d), "the rows and the pools differ in H_kv or D"
-    assert slot_mapping.shape == (k.shape[0],), "slot_mapping is [T]"
+    tokens, *row = k.shape
+    assert row == [h_kv, d], "the rows and the pools differ in H_kv or D"
+    assert slot_mapping.dim() == 1 and slot_mapping.numel() == tokens, "slot_mapping is [T]"
     dev = k_pages.device
     assert k.device == v.device == slot_mapping.device == dev, "tensors must be on the pools' device"
     quant = k_pages.dtype == torch.float8_e4m3fn and k.dtype != torch.float8_e4m3fn
@@ -161,7 +163,7 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
     with _lib.on_device(dev):
         _lib.check(_lib.load().fa4cp_paged_kv_write(
             k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k_pages.data_ptr(),
-            v_pages.data_ptr(), ks, vs, num_pages, page_size, slots.data_ptr(), k.shape[0], h_kv,
+            v_pages.data_ptr(), ks, vs, num_pages, page_size, slots.data_ptr(), tokens, h_kv,
             d, _lib.dtype_code(k.dtype), _lib.dtype_code(k_pages.dtype), _lib.ptr(kd),
             _lib.ptr(vd), _lib.stream_of(k_pages)), "paged_kv_write")
     _lib.count_launches()

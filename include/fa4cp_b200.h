@@ -584,14 +584,16 @@ FA4CP_API int fa4cp_paged_kv_accept(void* k_pages, void* v_pages, const int64_t*
  * Attention of a few new tokens a request over its paged cache: decode (one token) and the
  * verification of drafted trees.
  *   q            [total_q, Hq, D] at q_token_stride (elements); f16 | bf16 | e4m3
- *   K/V pools    as above; q's dtype, or e4m3 under any q
+ *   K/V pools    as above; q's dtype, or e4m3 under a bf16 q
  *   seq_lens     int32 [nseq]: cached tokens; the request's own n = cu_q[j+1] - cu_q[j] tokens
  *                are the last of them
  *   tree_mask    int64 [total_q, mask_words] (fa4cp_paged_tree_mask) or NULL: token i sees
  *                the new rows 0..i.  Every token sees all rows before the new ones.
  *   out, lse     [total_q, Hq, D] in q's dtype (bf16 for e4m3), [total_q, Hq] float32 natural
  *                log; rows that see no key: 0, -inf; rows outside cu_q are left as they are
- *   page_size    16, 32, 64 or a multiple of 128; a page outside [0, num_pages) reads zeros
+ *   page_size    16, 32, 64 or a multiple of 128; a page outside [0, num_pages) reads zeros,
+ *                rows behind the block table's last entry do not exist
+ *   max_seqlen_q upper bound on the requests' new tokens (sizes the launch that joins parts)
  *   *_descale    NULL or float32 [Hkv], each for an e4m3 operand only
  *   workspace    fa4cp_attn_paged_tree_workspace_bytes(...) bytes of scratch, 16-byte aligned
  *                (contents on entry do not matter; calls sharing it must not overlap)
