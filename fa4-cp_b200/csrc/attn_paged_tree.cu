@@ -1294,14 +1294,13 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 // 1 page), swizzled over `swizzle` bytes (0: not).
 int make_pool_map(CUtensorMap* map, const void* base, int num_pages, int page_size, int heads, int D,
                   int elem, const int64_t* strides, int rows, int inner, int swizzle) {
-  static EncodeTiledFn enc = nullptr;
-  if (enc == nullptr) {
+  static const EncodeTiledFn enc = []() -> EncodeTiledFn {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      enc = reinterpret_cast<EncodeTiledFn>(ptr);
-  }
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess;
+    return found ? reinterpret_cast<EncodeTiledFn>(ptr) : nullptr;
+  }();
   FA4CP_CHECK_ARG(enc != nullptr, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(page_size),
                               cuuint64_t(num_pages > 0 ? num_pages : 1)};

@@ -575,7 +575,7 @@ extern "C" int fa4cp_paged_kv_write(const void* k, const void* v, int64_t k_toke
   p.per_head = head_dim * se / 16;
   p.page_size = page_size;
   const int64_t columns = int64_t(num_heads_kv) * p.per_head;
-  FA4CP_CHECK_ARG(columns < (int64_t(1) << 24), "rows of %lld bytes are too long", (long long)columns * 16);
+  FA4CP_CHECK_ARG(columns < (int64_t(1) << 23), "rows of %lld bytes are too long", (long long)columns * 16);
   const int cols = int(columns < kWriteThreads ? columns : kWriteThreads);
   const int64_t groups = (num_tokens + kWriteThreads / cols - 1) / (kWriteThreads / cols);
   const int64_t parts = (columns + cols - 1) / cols;

@@ -371,3 +371,80 @@ def test_serving_loop(kv_dt):
         cached = paged_kv_accept(pools[0], pools[1], table, cached, acc.cuda(), cu_seqlens_q=plan.cu_seqlens_q)
         assert cached.tolist() == [r[0].shape[0] for r in rows]
     assert_device_ok()
+
+
+def test_write_descales_of_every_size():
+    """The stored value is e4m3 of the fp32 quotient for any divisor: tiny, huge, negative, 0 and
+    infinite ones, and subnormal ones."""
+    from fa4_ring import paged_kv_write
+    d = torch.tensor([0.0, math.inf, 1e-30, 1e30, 2.0 ** -60, -0.03, 1e-42, 3e38, 0.37, 2.0 ** 60])
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(40, 10, 64, generator=g) * torch.exp2(torch.randint(-11, 10, (40, 10, 64), generator=g).float())
+    near = torch.where(torch.isfinite(d) & (d != 0), d, 1.0)
+    x = (x.double() * near.double()[:, None]).to(BF)  # quotients over the whole of e4m3's range
+    x[0, :, :5] = torch.tensor([0.0, math.inf, -math.inf, math.nan, 2.0 ** 127]).to(BF)
+    pool = torch.zeros(3, 16, 10, 64, dtype=E4M3, device="cuda")
+    other = torch.zeros_like(pool)
+    paged_kv_write(x.cuda(), x.cuda(), pool, other, torch.arange(40).cuda(), k_descale=d.cuda(), v_descale=d.cuda())
+    want = (x.float() / d[:, None]).clamp(-448, 448).to(E4M3).float()
+    for p in (pool, other):
+        got = p.view(48, 10, 64)[:40].float().cpu()
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(want))
+    assert_device_ok()
+
+
+def test_write_rows_longer_than_a_block():
+    from fa4_ring import paged_kv_write
+    g = torch.Generator().manual_seed(11)
+    for hk, D, T in ((20, 256, 9), (33, 64, 700), (7, 24, 3)):
+        k, v = (torch.randn(T, hk, D, generator=g).to(F16).cuda() for _ in range(2))
+        slots = torch.randperm(T + 13, generator=g)[:T].cuda()
+        kp, vp = (torch.zeros(T + 13, 1, hk, D, dtype=F16, device="cuda") for _ in range(2))
+        paged_kv_write(k, v, kp, vp, slots)
+        assert torch.equal(kp[slots, 0], k) and torch.equal(vp[slots, 0], v)
+        assert int((kp != 0).any(-1).any(-1).sum()) == T
+    assert_device_ok()
+
+
+def test_accept_in_empty_pools():
+    from fa4_ring import paged_kv_accept
+    pool = torch.zeros(0, 16, 2, 128, dtype=BF, device="cuda")
+    lens = paged_kv_accept(pool, pool.clone(), i32([[-1], [-1]]), i32([4, 0]), i32([[1, 2], [0, 5]]),
+                           cu_seqlens_q=i32([0, 6, 7]))
+    assert lens.tolist() == [6, 1]
+
+
+def test_two_steps_at_once():
+    """Two requests sets, each written, planned and accepted on a stream of its own."""
+    from fa4_ring import paged_kv_accept, paged_kv_write
+    g = torch.Generator().manual_seed(13)
+    sets = []
+    for _ in range(2):
+        pools = [torch.randn(64, 16, 4, 128, generator=g).to(BF) for _ in range(2)]
+        rows = [torch.randn(96, 4, 128, generator=g).to(BF) for _ in range(2)]
+        slots = torch.randperm(1024, generator=g)[:96]
+        table = torch.randperm(64, generator=g)[:16].view(4, 4)
+        acc = torch.tensor([[1, 3, 5, 9]] * 4)
+        sets.append((pools, rows, slots, table, acc))
+
+    def step(s, stream):
+        (kp, vp), (k, v), slots, table, acc = s
+        with torch.cuda.stream(stream):
+            kp, vp = kp.cuda(), vp.cuda()
+            k, v, slots = k.cuda(), v.cuda(), slots.cuda()
+            table, acc = table.to(torch.int32).cuda(), acc.to(torch.int32).cuda()
+            cached, cu = i32([20, 3, 40, 11]), i32([0, 12, 24, 36, 48])
+            paged_kv_write(k, v, kp, vp, slots)
+            lens = paged_kv_accept(kp, vp, table, cached, acc, cu_seqlens_q=cu)
+        return kp, vp, lens
+
+    one = [step(s, torch.cuda.current_stream()) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        both = [step(s, st) for s, st in zip(sets, streams)]
+        torch.cuda.synchronize()
+        for a, b in zip(one, both):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    assert_device_ok()

@@ -372,6 +372,54 @@ def test_decode_agrees_with_paged_prefill_attention():
     ph.check_attn((out, lse), w)
 
 
+@pytest.mark.parametrize("n,group,D,kv_dt", [(33, 4, 128, E4M3), (64, 8, 64, E4M3), (130, 3, 256, E4M3), (3, 160, 128, BF),
+                                             (1, 300, 64, F16), (2, 129, 256, E4M3)])
+def test_several_row_tiles(n, group, D, kv_dt):
+    """More rows than a tile holds: many tokens, or more query heads of one K/V head than that."""
+    q_dt = F16 if kv_dt == F16 else BF
+    x = make([n, n + 300, n + 77], [n, max(n // 2, 1), n], group, 1, D, q_dt, kv_dt, 32, seed=n + group)
+    ph.check_attn(call(x), want(x))
+    assert_device_ok()
+
+
+@pytest.mark.parametrize("kv_dt,D", [(BF, 128), (E4M3, 64), (E4M3, 256)])
+def test_many_row_tiles_of_a_block(kv_dt, D):
+    """Some 20 short row tiles for every SM: the ring in which the items are passed on wraps."""
+    lens = [1 + (11 * i) % 90 for i in range(750)]
+    x = make(lens, [1] * 750, 4, 4, D, BF, kv_dt, 16, seed=D, tree=False)
+    ph.check_attn(call(x), want(x))
+    assert_device_ok()
+
+
+def test_requests_that_share_pages():
+    """A prefix held once: the first pages of two requests are the same."""
+    x = make([200, 200], [5, 3], 8, 2, 128, BF, BF, 32, seed=16)
+    x["table"][1, :5] = x["table"][0, :5]
+    ph.check_attn(call(x), want(x))
+
+
+def test_two_calls_at_once():
+    from fa4_ring import b200_attn_paged_tree
+    xs = [make([3000, 40, 700], [7, 1, 12], 8, 2, 128, BF, kv_dt, 64, seed=17) for kv_dt in (BF, E4M3)]
+    one = [call(x) for x in xs]
+    args = []
+    for x in xs:
+        args.append(((dev(x["q"]), dev(x["k"]), dev(x["v"]), dev(x["table"])), dict(
+            cu_seqlens_q=dev(x["cu"]), seq_lens=torch.tensor(x["lens"], dtype=torch.int32).cuda(),
+            max_seqlen_q=12, tree_mask=dev(x["mask"]), k_descale=dev(x["kd"]), v_descale=dev(x["vd"]))))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    for _ in range(5):
+        both = []
+        for (a, kw), st in zip(args, streams):
+            with torch.cuda.stream(st):
+                both.append(b200_attn_paged_tree(*a, **kw))
+        torch.cuda.synchronize()
+        for a, b in zip(one, both):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    assert_device_ok()
+
+
 def test_refusals():
     x = make([40], [2], 4, 2, 128, BF, BF, 16, seed=16)
     for change, err in ((dict(page=24), ValueError), (dict(d=96), NotImplementedError)):
