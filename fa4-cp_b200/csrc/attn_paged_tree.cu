@@ -11,7 +11,7 @@
 //
 // Schedule.  The work is the list of all (request, K/V head, row tile, key tile), in that
 // order; every CTA takes an equal share of consecutive key tiles, whatever the lengths are
-// (they are only known on the device).  A row tile counts kItemCost tiles more than it has, for
+// (they are only known on the device).  A row tile counts ITEM_COST tiles more than it has, for
 // its Q and its result.  A row tile whose keys several CTAs share leaves one partial (O, m, l)
 // each in the workspace, joined by tree_combine_kernel in a fixed order.  A CTA has at most two
 // partials (its first and its last row tile), so the workspace does not depend on the lengths.
@@ -73,7 +73,6 @@ enum : int {
   kErrItemFree, kErrQStaged, kErrDrain
 };
 
-constexpr int kItemCost = 6;  // key tiles that a row tile's start and end are worth
 constexpr int kItems = 8;     // ring of items
 
 // A CTA's part of a row tile, as the roles of a CTA pass it on (nt == 0: the share has ended).
@@ -106,6 +105,10 @@ template <int D_, bool KV8_>
 struct TreeTraits {
   static constexpr int D = D_, BN = D == 256 ? 32 : 64;  // keys of a tile
   static constexpr bool KV8 = KV8_;
+  // key tiles that a row tile's start and end are worth: a tile of an e4m3 cache takes less of a
+  // CTA's time (32 requests, 64 tokens: e4m3 D128 352 us with 6, 348 with 9, 341 with 12; bf16 386,
+  // 380, 384)
+  static constexpr int ITEM_COST = KV8 ? 12 : 8;
   static constexpr int KEL = KV8 ? 1 : 2;             // bytes of a K element
   static constexpr int K_SWZ = D * KEL >= 128 ? 128 : 64;  // bytes of a swizzled row of K
   static constexpr int K_COLS = D * KEL / K_SWZ;
@@ -211,7 +214,7 @@ __device__ __forceinline__ Request load_request(const TreeParams& p, int j) {
   return r;
 }
 
-// Tiles are counted with kItemCost more for every row tile: `total` of them, of which CTA c of
+// Tiles are counted with ITEM_COST more for every row tile: `total` of them, of which CTA c of
 // g takes the c-th equal part.
 struct Share {
   int64_t t0, t1;        // this CTA's part
@@ -239,7 +242,7 @@ struct Start {
 // All threads of the CTA.  A thread sums a run of requests, a block scan gives its run's first
 // tile, and the thread whose run holds t0 finds the request and leaves it in `found`.  (All this
 // is a small batch's latency: each wait for global memory takes 700 cycles or so.)
-template <int BN, int THREADS>
+template <int BN, int COST, int THREADS>
 __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, int64_t* ws, Start* found) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (p.nseq + THREADS - 1) / THREADS;
@@ -249,7 +252,7 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
 #pragma unroll 1
   for (int j = j0; j < j1; ++j) {
     r = load_request<BN>(p, j);
-    sum += int64_t(p.Hkv * r.mt) * (r.kt + kItemCost);
+    sum += int64_t(p.Hkv * r.mt) * (r.kt + COST);
   }
   int64_t inc = sum;
 #pragma unroll
@@ -278,7 +281,7 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
 #pragma unroll 1
     for (int j = j0; j < j1; ++j) {
       if (per > 1) r = load_request<BN>(p, j);
-      const int64_t tiles = int64_t(p.Hkv * r.mt) * (r.kt + kItemCost);
+      const int64_t tiles = int64_t(p.Hkv * r.mt) * (r.kt + COST);
       if (s.t0 < first + tiles) {
         found->r = r;
         found->seq = j;
@@ -293,7 +296,7 @@ __device__ __forceinline__ Share find_share(const TreeParams& p, int c, int G, i
 }
 
 // Walks a CTA's share item by item (warp 8).
-template <int BN>
+template <int BN, int COST>
 struct Walk {
   Request r;
   int64_t left;         // counted tiles left of the share, from the current position on
@@ -303,8 +306,8 @@ struct Walk {
     seq = f.seq;
     left = s.t1 - s.t0;
     r = f.r;
-    const int64_t item = quotient(f.off, r.kt + kItemCost);
-    at = int(f.off - item * (r.kt + kItemCost));
+    const int64_t item = quotient(f.off, r.kt + COST);
+    at = int(f.off - item * (r.kt + COST));
     kvh = int(item) / r.mt;
     mtile = int(item) - kvh * r.mt;
   }
@@ -312,9 +315,9 @@ struct Walk {
   __device__ __forceinline__ bool next(const TreeParams& p) {
     while (left > 0) {
       if (r.n > 0) {
-        const int here = int(min(int64_t(r.kt + kItemCost - at), left));
-        kt0 = max(at - kItemCost, 0);
-        nt = max(at + here - kItemCost, 0) - kt0;
+        const int here = int(min(int64_t(r.kt + COST - at), left));
+        kt0 = max(at - COST, 0);
+        nt = max(at + here - COST, 0) - kt0;
         left -= here;
         at = 0;
         if (nt > 0) return true;
@@ -519,7 +522,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
   // fills the ring)
   int64_t* sched = reinterpret_cast<int64_t*>(smem);
   Start* found = reinterpret_cast<Start*>(sched + 32);
-  const Share share = find_share<BN, TR::THREADS>(p, cta, int(gridDim.x), sched, found);
+  const Share share = find_share<BN, TR::ITEM_COST, TR::THREADS>(p, cta, int(gridDim.x), sched, found);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
@@ -625,7 +628,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
                          mbar_wait(BAR(first_full + slots + int(slot)), ph ^ 1, abort, kErrEmpty, status);
         return __all_sync(0xffffffffu, got);
       };
-      Walk<BN> w;
+      Walk<BN, TR::ITEM_COST> w;
       bool more = true;
       if (!is_v) {
         w.start(*found, share);
