@@ -146,8 +146,10 @@ struct TreeTraits {
   static_assert(KS < 2 * kItems, "Q staging ring");
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int SMEM_BYTES = OFF_MISC + 128 + 1024;
-  // an e4m3 V tile is widened by one warp (two at head_dim 256), the next tile by the next
-  static constexpr int CONV_WARPS = KV8 ? 4 : 0, CONV_TEAM = D == 256 ? 2 : 1;
+  // an e4m3 V tile is widened by all four warps, by two at head_dim 64, where it is half as large:
+  // their load on the exponential unit then spreads over the SM's quarters, and no softmax warp is
+  // later than the others (a warp a tile: D128, 64 tokens and one 347 and 172 us, so 341 and 156)
+  static constexpr int CONV_WARPS = KV8 ? 4 : 0, CONV_TEAM = D == 64 ? 2 : 4;
   static constexpr int THREADS = W0 * 32 + 128 + CONV_WARPS * 32;
   // setmaxnreg split, in registers a thread of a warpgroup; the launch gives 512 x 128 or
   // 384 x 168 registers
