@@ -329,7 +329,8 @@ def b200_attn_paged_tree(
         assert tree_mask.device == dev, "tree_mask must be on q's device"
         words = tree_mask.shape[1]
         tree_mask = tree_mask.contiguous()
-    qd, kd, vd = (norm_descale(d, h_kv, dev) for d in (q_descale, k_descale, v_descale))
+    qd, kd = norm_descale(q_descale, h_kv, dev), norm_descale(k_descale, h_kv, dev)
+    vd = norm_descale(v_descale, h_kv, dev)
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
     q = rows16(q)

@@ -92,7 +92,8 @@ def paged_block_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor,
     if num_free is not None:
         num_free = as_i32(num_free, dev)
         assert num_free.numel() == 1, "num_free is one number"
-    cached_lens, new_lens, free_pages = (as_i32(t, dev) for t in (cached_lens, new_lens, free_pages))
+    cached_lens, new_lens = as_i32(cached_lens, dev), as_i32(new_lens, dev)
+    free_pages = as_i32(free_pages, dev)
     table = cached_lens.new_empty((nseq, max_pages))
     slots = cached_lens.new_empty(num_tokens, dtype=torch.int64)
     cu_q, cu_k, lens, pages = cached_lens.new_empty(3 * nseq + 4).unsafe_split_with_sizes(
@@ -191,7 +192,8 @@ def paged_kv_accept(k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: t
     assert accepted.dim() == 2 and accepted.shape[0] == nseq, "accepted is [nseq, A]"
     assert cu_seqlens_q.numel() == nseq + 1, "cu_seqlens_q is [nseq + 1]"
     ks, vs = pool_strides(k_pages, "k_pages"), pool_strides(v_pages, "v_pages")
-    bt, cached, acc, cu = (as_i32(t, dev) for t in (block_table, cached_lens, accepted, cu_seqlens_q))
+    bt, cached = as_i32(block_table, dev), as_i32(cached_lens, dev)
+    acc, cu = as_i32(accepted, dev), as_i32(cu_seqlens_q, dev)
     lens = cached.new_empty(nseq)
     with _lib.on_device(dev):
         _lib.check(_lib.load().fa4cp_paged_kv_accept(
