@@ -8,10 +8,10 @@
 // are packed into rows of one 128-row MMA tile (row = token * group + head of the group), and
 // K and V are read once for all of them.
 //
-// Measured (32/8 heads, head_dim 128).  64 decoding requests of 1K to 32K tokens, bf16: 0.67 to
-// 0.74 ms = 6.0 to 6.6 TB/s, the rate of a copy.  32 requests of up to 16K tokens: bf16 with 1, 8
+// Measured (32/8 heads, head_dim 128).  64 decoding requests of 1K to 32K tokens, bf16: 0.68 to
+// 0.72 ms = 6.2 to 6.5 TB/s, the rate of a copy.  32 requests of up to 16K tokens: bf16 with 1, 8
 // and 32 new tokens 180, 190 and 200 us (5.3 to 6.1 TB/s); 64 tokens are two row tiles, 381 us
-// (630 TFLOP/s).  Over an e4m3 cache 1 and 64 tokens take 155 and 341 us: a key tile of a CTA
+// (630 TFLOP/s).  Over an e4m3 cache 1 and 64 tokens take 150 and 336 us: a key tile of a CTA
 // takes 1000 to 1100 cycles whatever its bytes, the round trip of an S buffer (S 430, softmax 1810,
 // P to PV 210, PV 600, next S 370 cycles) over the three buffers that TMEM leaves.  One request of
 // 100 and 8K tokens: 11 and 18 us, mostly launch and start.
