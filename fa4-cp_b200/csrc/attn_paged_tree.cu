@@ -78,7 +78,7 @@ constexpr int BM = 128;
 // codes written to the device status word when a bounded wait gives up
 enum : int {
   kErrEmpty = 0x401, kErrRawFull, kErrVEmpty, kErrQFull, kErrKFull, kErrPFull,
-  kErrVFull, kErrOFree, kErrSFull, kErrSFree, kErrMax, kErrODone, kErrVFix, kErrJoin, kErrMeet, kErrItem,
+  kErrVFull, kErrOFree, kErrSFull, kErrSFree, kErrMax, kErrODone, kErrVFix, kErrJoin, kErrItem,
   kErrItemFree, kErrQStaged, kErrDrain
 };
 
@@ -126,7 +126,9 @@ struct TreeTraits {
   static constexpr int V_CHUNK = BN * 128;
   static constexpr int V_BYTES = BN * D * 2;
   static constexpr int RAW_BYTES = BN * D;            // one e4m3 V tile
-  static constexpr int KS = KV8 && D == 256 ? 8 : 6, VS = 6, RS = KV8 ? 6 : 0;
+  // ring slots: what shared memory holds, 8 at head_dim 64 (e4m3, 64 tokens and one: 273 and 140 us,
+  // with 6 276 and 143, with 12 288 and 148)
+  static constexpr int KS = D == 64 || (KV8 && D == 256) ? 8 : 6, VS = D == 64 ? 8 : 6, RS = KV8 ? VS : 0;
   static_assert(KS * K_BYTES >= BM * D * 2, "the K ring takes the Q of an item whole");
   static constexpr int OFF_V = KS * K_BYTES;
   static constexpr int OFF_RAW = OFF_V + VS * V_BYTES;
@@ -412,7 +414,8 @@ __device__ __forceinline__ void q16_terms(const uint4 a, const uint4 b, float f,
 
 // Rows that see a key whose V row is not finite, after the finite part has been written to
 // their row of the result (16-bit) or of a partial (fp32): the non-finite values themselves are
-// added (their weight is positive): of every STEP blocks of 16 columns the one at `first`.  Rare; reads V again from the pool.
+// added (their weight is positive): of every STEP blocks of 16 columns the one at `first`.  Rare;
+// reads V again from the pool.
 template <int D, int STEP>
 __device__ __forceinline__ void add_nonfinite(const TreeParams& p, int seq, int kvh, int ctx, int lim,
                                               int64_t tok, int node, int key0, int key1, int first,
