@@ -324,9 +324,9 @@ constexpr int kWriteThreads = 256, kWriteBlocks = 4, kWriteBatch = 2;
 // A thread owns 16 bytes of the source row's columns, in K and in V, and takes a token out of
 // every `gridDim.x` groups of them.  QUANT: 0 copy, 1 bf16 -> e4m3, 2 f16 -> e4m3.  Bound by
 // memory: a row's loads do not wait for its slot, which decides on the store alone.  Measured:
-// 65536 rows of 8 heads x 128, bf16 into e4m3, 73.5 us = 5.5 TB/s (62.4 us at the rate of a
-// copy); a thread a token instead of the loop 93 us, batches of 4 at 64 registers (spills) 86 us,
-// at 80 registers (3 blocks) 77 us.  64 rows: 1.7 us, the launch.
+// 65536 rows of 8 heads x 128, bf16 into e4m3, 71.5 us = 5.6 TB/s (62.4 us at the rate of a
+// copy); loads marked as streaming 73.5 us, a thread a token instead of the loop 93 us, batches of
+// 4 at 64 registers (spills) 86 us, at 80 registers (3 blocks) 77 us.  64 rows: 1.7 us, the launch.
 template <int QUANT>
 __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(const WriteParams p) {
   const int cols = min(p.heads * p.per_head, kWriteThreads);  // of a block
@@ -354,8 +354,8 @@ __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(c
       slot[i] = -1;
       if (t < p.tokens) {
         slot[i] = p.slots[t];
-        k[i] = __ldcs(reinterpret_cast<const uint4*>(ks + t * p.k_stride));
-        v[i] = __ldcs(reinterpret_cast<const uint4*>(vs + t * p.v_stride));
+        k[i] = *reinterpret_cast<const uint4*>(ks + t * p.k_stride);
+        v[i] = *reinterpret_cast<const uint4*>(vs + t * p.v_stride);
       }
     }
 #pragma unroll
@@ -400,7 +400,7 @@ struct AcceptParams {
 // from and goes to) are worked out once, a thread each; then a thread owns a column of K or of V
 // through all of them.  The list ascends, so node a_i >= i: a batch of loads followed by its
 // stores never overwrites a row that a later batch reads.  Bound by three dependent reads (list,
-// table, rows) and, for many requests, by the rows: with the write of 16384 new rows 19 us for 256
+// table, rows) and, for many requests, by the rows: with the write of 16384 new rows 18 us for 256
 // requests whose 12 rows move over an e4m3 cache (13.5 us of traffic); 26 us when every thread
 // worked the moves out for itself.
 __global__ void __launch_bounds__(kAcceptThreads) kv_accept_kernel(const AcceptParams p) {
