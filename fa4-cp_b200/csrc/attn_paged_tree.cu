@@ -1112,6 +1112,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
               if (hit) *at = make_uint4(y[0], y[1], y[2], y[3]);
             }
           }
+          __syncwarp();
           fence_async_shared();
           if (x.n > 1) {
             // which keys of the tile were cleared: one word a warp, two sets used in turn
@@ -1202,20 +1203,22 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           }
 #pragma unroll
           for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * mult;
-          if (!valid) continue;
-          if (whole) {
-            uint32_t h[8];
+          if (valid) {
+            if (whole) {
+              uint32_t h[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              h[e] = p.out_bf16 ? pack_bf16x2(f[2 * e], f[2 * e + 1]) : pack_f16x2(f[2 * e], f[2 * e + 1]);
-            uint4* dst = reinterpret_cast<uint4*>(out_row + c * 16);
-            dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
-            dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
-          } else {
-            float4* dst = reinterpret_cast<float4*>(prow + c * 16);
+              for (int e = 0; e < 8; ++e)
+                h[e] = p.out_bf16 ? pack_bf16x2(f[2 * e], f[2 * e + 1]) : pack_f16x2(f[2 * e], f[2 * e + 1]);
+              uint4* dst = reinterpret_cast<uint4*>(out_row + c * 16);
+              dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+              dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+            } else {
+              float4* dst = reinterpret_cast<float4*>(prow + c * 16);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) __stcg(dst + e, make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]));
+              for (int e = 0; e < 4; ++e) __stcg(dst + e, make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]));
+            }
           }
+          __syncwarp();  // the next loads from TMEM are the whole warp's
         }
       }
       warp_arrive(o_free);
