@@ -1087,16 +1087,18 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         }
         if (edge) {
           // P is 0 where a row does not look, but 0 * NaN is NaN: V rows behind the cache are
-          // cleared, and so are the non-finite values of new rows (a context row is seen by
-          // every token, so its values go through as they are).  Thread t has key t % BN, and its
-          // share of the columns.
+          // cleared, and so are the non-finite values of new rows that some token may not see (a
+          // context row is seen by every token, and one token without a mask sees itself, so
+          // their values go through as they are).  Thread t has key t % BN, and its share of the
+          // columns.
+          const bool hides = x.n > 1 || p.mask != nullptr;
           ok = mbar_wait(v_full(it), phase(it, TR::VS), abort, kErrVFix, status);
           if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
           constexpr int PER = D / 8 * BN / 128;  // 16-byte pieces of a thread
           const int key = kbase + (t & (BN - 1));
           uint8_t* vrow = smem + TR::OFF_V + (it % TR::VS) * TR::V_BYTES + (t & (BN - 1)) * 128;
           bool mine_bad = false;
-          if (key >= x.lim || (key >= ctx && x.n > 1)) {
+          if (key >= x.lim || (key >= ctx && hides)) {
 #pragma unroll 1
             for (int c = t / BN * PER; c < (t / BN + 1) * PER; ++c) {
               uint4* at = reinterpret_cast<uint4*>(vrow + (c >> 3) * TR::V_CHUNK + (c & 7) * 16);
@@ -1114,7 +1116,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           }
           __syncwarp();
           fence_async_shared();
-          if (x.n > 1) {
+          if (hides) {
             // which keys of the tile were cleared: one word a warp, two sets used in turn
             const uint32_t word = __ballot_sync(0xffffffffu, mine_bad);
             volatile uint32_t* set = bad + wg * 8 + (fixes & 1) * 4;

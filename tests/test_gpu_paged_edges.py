@@ -28,3 +28,31 @@ def test_partly_filled_warps(kv_dt, D, rows):
     x = make([90, rows + 3000], [rows, rows], 1, 1, D, q_dt, kv_dt, 32, seed=rows + D)
     ph.check_attn(call(x), want(x))
     assert_device_ok()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("kv_dt,D", [(BF, 128), (F16, 64), (E4M3, 128), (BF, 256), (E4M3, 256)])
+def test_one_token_that_does_not_see_itself(kv_dt, D, bad):
+    """A request of one token whose mask hides the token's own row: whatever the row holds stays out,
+    over a cache and over none."""
+    if kv_dt == E4M3 and not math.isnan(bad):
+        pytest.skip("e4m3 has no infinities")
+    x = make([1, 70, 1300], [1, 1, 1], 4, 2, D, F16 if kv_dt == F16 else BF, kv_dt, 16, seed=D)
+    for j, n in enumerate(x["lens"]):
+        x["seen"][j][0] = False
+        x["mask"][j] = 0
+        page = int(x["table"][j, (n - 1) // 16])
+        for name in ("k", "v"):
+            pool = x[name].float()
+            pool[page, (n - 1) % 16] = bad
+            x[name] = pool.to(kv_dt)
+    out, lse = call(x)
+    assert bool((out[0] == 0).all()) and bool((lse[0] == -math.inf).all())
+    ph.check_attn((out, lse), want(x))
+    # a mask that shows the row again
+    x["seen"][1][0] = True
+    x["mask"][1] = 1
+    out, lse = call(x)
+    assert not torch.isfinite(out[1].float()).any()
+    ph.check_attn((out, lse), want(x), torch.tensor([True, False, True]))
+    assert_device_ok()
