@@ -72,7 +72,15 @@ int tree_status(int* value, bool clear) {
 namespace {
 
 constexpr float kNegInf = -__builtin_huge_valf();
-constexpr float kRescaleThreshold = 8.0f;  // log2 units: P <= 256
+constexpr float kRescaleThreshold = 8.0f;  // log2 units: P <= 256 times the largest at its maximum
+// P is rounded to the 16-bit type of the V that it multiplies (f16 for an e4m3 V), by half a step:
+// 2^-8 of each weight in bf16, 2^-11 in f16.  (Both operands of an MMA are of one type; bf16 over a
+// bf16 cache, 64 requests of 1K to 32K tokens: 0.0023 off the 64-bit result, all in 32 bits 0.0017,
+// which is the output's own rounding.)  An f16 also ends at the bottom: it is subnormal below
+// 2^-14 and 0 below 2^-25, while the sum of the weights is in 32 bits and keeps them all.  So an f16 P
+// carries a factor of 2^7, which the sum and O share: the largest weight is between 2^7 and 2^15, and
+// what is lost of a weight is below 2^-32 of it.
+constexpr float kLiftF16 = 7.0f;
 constexpr int BM = 128;
 
 // codes written to the device status word when a bounded wait gives up
@@ -102,7 +110,7 @@ struct TreeParams {
   float* lse;
   const float *q_descale, *k_descale, *v_descale;
   float* part_o;   // [2 * grid][BM][D]
-  float2* part_ml; // [2 * grid][BM]: running maximum (log2 units, scaled), sum
+  float2* part_ml; // [2 * grid][BM]: what the exponents are relative to (log2 units), sum
   int4* desc;      // [grid][2]: the row tile whose first part a CTA holds
   int64_t total_q;
   int nseq, Hq, Hkv, group, page_size, num_pages, max_pages, mask_words;
@@ -981,6 +989,12 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         scale /= qf;
         scale = scale < 1.17549435e-38f ? 1.17549435e-38f : scale;
       }
+      // What a row's exponents (log2 units) are relative to, given its maximum.  Rounded upwards for
+      // an f16 P, so that no rounding of a large maximum takes P past 2^15; sums and O are brought
+      // from one maximum to another by the difference of these same numbers.
+      auto offset = [&](float mx) -> float {
+        return !TR::KV8 && bf16_op ? mx * scale : __fmaf_ru(mx, scale, -kLiftF16);
+      };
       // m: the maximum that this warpgroup's sum l (and its O) are relative to
       float m = kNegInf, l = 0.f;
       bool sees_bad = false;
@@ -1043,12 +1057,12 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           }
           // from here on off the other warpgroup's way
           if (m_new != m) {
-            if (m != kNegInf) l *= ex2_approx((m - m_new) * scale);
+            if (m != kNegInf) l *= ex2_approx(offset(m) - offset(m_new));
             m = m_new;
           }
           constexpr int MINE = TR::APART ? NWG : 1;  // PV(it - MINE) was the last one into this O
           if (j >= MINE && __any_sync(0xffffffffu, raise)) {
-            const float f = !raise ? 1.f : so_far == kNegInf ? 0.f : ex2_approx((so_far - m_new) * scale);
+            const float f = !raise ? 1.f : so_far == kNegInf ? 0.f : ex2_approx(offset(so_far) - offset(m_new));
             ok = mbar_wait(o_done(it - MINE), phase(it - MINE, NB), abort, kErrODone, status);
             if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
             tc_fence_after();
@@ -1064,7 +1078,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
             }
           }
           // (P = 0 in a lane without a row, for the same reason)
-          const float neg_m = !valid ? kNegInf : (m == kNegInf) ? 0.f : -m * scale;
+          const float neg_m = !valid ? kNegInf : (m == kNegInf) ? 0.f : -offset(m);
           const uint64_t scale2 = f2pack(scale, scale), negm2 = f2pack(neg_m, neg_m);
           uint64_t rs[2] = {0ull, 0ull};
           uint32_t pw[C][16];
@@ -1170,7 +1184,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
 #pragma unroll
       for (int g = 0; g < NWG; ++g) {
         const float lg = end_sum[(set + g) * BM + t], mg = part_f[g];
-        part_f[g] = mg == m ? 1.f : mg == kNegInf ? 0.f : ex2_approx((mg - m) * scale);
+        part_f[g] = mg == m ? 1.f : mg == kNegInf ? 0.f : ex2_approx(offset(mg) - offset(m));
         l += mg == kNegInf ? lg : lg * part_f[g];  // (NaN sums have no maximum)
         sees_bad |= end_bad[(set + g) * BM + t] != 0;
       }
@@ -1225,7 +1239,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       }
       warp_arrive(o_free);
       if (valid) {
-        const float ms = m == kNegInf ? kNegInf : m * scale;  // log2 units
+        const float ms = m == kNegInf ? kNegInf : offset(m);
         if (wg == 0) {
           if (whole) p.lse[tok * p.Hq + head] = l == 0.f ? kNegInf : (ms + lg2_approx(l)) * kLn2;
           else __stcg(&p.part_ml[part * BM + t], make_float2(ms, l));

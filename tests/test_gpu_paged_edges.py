@@ -56,3 +56,73 @@ def test_one_token_that_does_not_see_itself(kv_dt, D, bad):
     assert not torch.isfinite(out[1].float()).any()
     ph.check_attn((out, lse), want(x), torch.tensor([True, False, True]))
     assert_device_ok()
+
+
+@pytest.mark.parametrize("q_dt,kv_dt", [(F16, F16), (BF, E4M3), (E4M3, E4M3)], ids=["f16", "bf16-e4m3", "e4m3"])
+@pytest.mark.parametrize("D,gap", [(64, 16), (64, 18), (64, 20), (128, 18), (256, 18)])
+def test_weights_far_below_the_largest(q_dt, kv_dt, D, gap):
+    """A few keys `gap` above all others, with values of 0: the others make the result.
+
+    P is an f16 with its largest at 2^7 or more, so a weight is off by at most half of f16's least
+    value, 2^-25, of 2^7 of the largest: m 2^-32 in all, beside the relative errors that
+    paged_helpers.attn derives.  (Only the keys of one CTA share a largest P, so there are as many
+    requests as two for each CTA, over the same pages.)"""
+    from fa4_ring import b200_attn_paged_tree
+    n, page, batch = 16384, 128, 296
+    scale = 1.0 / D
+    top = torch.tensor(gap / 4.0)  # q = 4, K = gap / 4: a score of gap; both are e4m3 values
+    assert float(top.to(E4M3)) == float(top)
+    k, v = torch.zeros(n, 1, D), torch.ones(n, 1, D)
+    strong = torch.arange(0, 256, 32)  # of either warpgroup's tiles
+    k[strong], v[strong] = top, 0.0
+    q = torch.full((batch, 4, D), 4.0)
+    k, v = (t.view(n // page, page, 1, D).to(kv_dt).cuda() for t in (k, v))
+    table = torch.arange(n // page, dtype=torch.int32).expand(batch, -1).contiguous().cuda()
+    out, lse = b200_attn_paged_tree(
+        q.to(q_dt).cuda(), k, v, table, cu_seqlens_q=torch.arange(batch + 1, dtype=torch.int32).cuda(),
+        seq_lens=torch.full((batch,), n, dtype=torch.int32).cuda(), max_seqlen_q=1, softmax_scale=scale)
+    rest, few = n - len(strong), len(strong)
+    total = few + rest * math.exp(-gap)
+    exact = rest * math.exp(-gap) / total
+    e = (D + 8) * 2.0 ** -24 * gap
+    if kv_dt == E4M3 and q_dt != E4M3:
+        e += 2.0 ** -17 * scale * 4.0 * D * gap / 4.0
+    rel = 2.0 ** -11 + 2 * (2 * e + 2.0 ** -20) + (n + 8) * 2.0 ** -24
+    u_o = 2.0 ** -11 if q_dt == F16 else 2.0 ** -8
+    tol = rel * exact + n * 2.0 ** -32 + 2 * u_o * exact + 2.0 ** -25
+    err = (out.double() - exact).abs().max().item()
+    assert err <= tol, f"off by {err:.3e} of {exact:.3e}, allowed {tol:.3e}"
+    want_lse = gap + math.log(total)
+    err = (lse.double() - want_lse).abs().max().item()
+    assert err <= 2 * e + 2.0 ** -20 + n * 2.0 ** -24 + 2.0 ** -22 * want_lse
+    assert_device_ok()
+
+
+@pytest.mark.parametrize("q_dt,kv_dt", [(F16, F16), (BF, BF)])
+@pytest.mark.parametrize("D,tile", [(64, 64), (128, 64), (256, 32)])
+def test_scores_past_the_steps_of_32_bits(q_dt, kv_dt, D, tile):
+    """Scores of 2^26 in log2 units, where fp32 counts in steps of 4 and 8: the second half of the
+    keys is 8 above the first, the most by which a maximum is left as it is.  The scores and their
+    differences are exact, so the weights 1 and 256 are."""
+    from fa4_ring import b200_attn_paged_tree
+    n, batch = 4 * tile, 444  # as many requests as give a CTA whole ones
+    k = torch.zeros(n, 1, D)
+    k[:, 0, 0] = 4096.0
+    k[n // 2:, 0, 1] = 2.0
+    v = torch.zeros(n, 1, D)
+    v[n // 2:, 0, ::2] = 1.0
+    v[:n // 2, 0, 1::2] = 1.0
+    q = torch.zeros(batch, 1, D)
+    q[:, 0, 0], q[:, 0, 1] = 4096.0, 1.0
+    table = torch.arange(n // 32, dtype=torch.int32).expand(batch, -1).contiguous().cuda()
+    out, lse = b200_attn_paged_tree(
+        q.to(q_dt).cuda(), k.view(-1, 32, 1, D).to(kv_dt).cuda(), v.view(-1, 32, 1, D).to(kv_dt).cuda(), table,
+        cu_seqlens_q=torch.arange(batch + 1, dtype=torch.int32).cuda(),
+        seq_lens=torch.full((batch,), n, dtype=torch.int32).cuda(), max_seqlen_q=1, softmax_scale=4 * math.log(2))
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    # the weights are powers of two (exact in P), the hardware exponential is good to 2^-20, the scale to
+    # 2^-23 of 8, and the result is rounded once
+    for part, exact in ((out[..., ::2], 256 / 257), (out[..., 1::2], 1 / 257)):
+        tol = exact * (ph.HALF_STEP[q_dt] + 2.0 ** -18)
+        assert (part.double() - exact).abs().max().item() <= tol
+    assert_device_ok()
