@@ -258,13 +258,14 @@ def pool_strides(pool: torch.Tensor, what: str):
 
 def rows16(x: torch.Tensor) -> torch.Tensor:
     """``x [T, H, D]`` as rows of ``H * D`` dense elements at a 16-byte aligned token stride:
-    a slice of a fused projection is taken as it is, anything else is copied."""
+    a slice of a fused projection is taken as it is, anything else is copied (dense rows at an
+    address that is not aligned, too, which ``contiguous`` would give back as they are)."""
     _, heads, d = x.shape
     token, head, elem = x.stride()
     if (elem == 1 and (head == d or heads == 1)
             and (token * x.element_size() | x.data_ptr()) & 15 == 0):
         return x
-    return x.contiguous()
+    return x.clone(memory_format=torch.contiguous_format)
 
 
 def as_i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:

@@ -126,3 +126,30 @@ def test_scores_past_the_steps_of_32_bits(q_dt, kv_dt, D, tile):
         tol = exact * (ph.HALF_STEP[q_dt] + 2.0 ** -18)
         assert (part.double() - exact).abs().max().item() <= tol
     assert_device_ok()
+
+
+def test_unaligned_rows_of_one_token():
+    """One token at an address that is not 16-byte aligned, dense as it is, is copied like any other
+    view: a slice of a fused projection, and rows at an odd offset of a flat buffer."""
+    from fa4_ring import paged_kv_write
+    for new in ([1], [1, 4]):
+        T = sum(new)
+        x = make([70 + n for n in new], new, 8, 2, 128, BF, BF, 32, seed=31, tree=False)
+        ref = call(x)
+        odd = torch.zeros(T, 8 * 128 + 3, dtype=BF, device="cuda")
+        odd[:, 3:] = x["q"].reshape(T, -1).cuda()
+        flat = torch.zeros(1 + T * 8 * 128, dtype=BF, device="cuda")
+        flat[1:] = x["q"].reshape(-1).cuda()
+        for q in (odd[:, 3:].view(T, 8, 128), flat[1:].view(T, 8, 128)):
+            assert q.data_ptr() % 16
+            got = call(x, q=q)
+            assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+        slots = torch.arange(T).cuda() + 5
+        rows = torch.randn(2, T, 2, 128, generator=torch.Generator().manual_seed(3)).to(BF).cuda()
+        wide = torch.zeros(T, 1 + 512, dtype=BF, device="cuda")
+        wide[:, 1:] = rows.permute(1, 0, 2, 3).reshape(T, 512)
+        k, v = (wide[:, 1 + 256 * i:257 + 256 * i].view(T, 2, 128) for i in (0, 1))
+        pools = torch.zeros(2, 2, 16, 2, 128, dtype=BF, device="cuda")
+        paged_kv_write(k, v, pools[0], pools[1], slots)
+        assert torch.equal(pools.view(2, 32, 2, 128)[:, 5:5 + T], rows)
+    assert_device_ok()

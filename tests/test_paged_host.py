@@ -1,0 +1,30 @@
+"""Host side of the paged-cache wrappers (no GPU needed)."""
+
+import pytest
+import torch
+
+BF, F16, E4M3 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+def _aligned(n, dt):
+    """A flat buffer of n elements at a 16-byte aligned address."""
+    x = torch.arange(n + 16, dtype=torch.float32).to(dt)
+    skip = -x.data_ptr() % 16 // x.element_size()
+    return x[skip:skip + n]
+
+
+@pytest.mark.parametrize("dt", [BF, F16, E4M3])
+@pytest.mark.parametrize("T,H,D", [(1, 1, 64), (1, 4, 64), (3, 4, 64), (2, 1, 128)])
+def test_rows_end_up_aligned(dt, T, H, D):
+    from fa4_ring.attn_backend import rows16
+    base = _aligned(T * H * D + 16 + 32 * T, dt)
+    n = T * H * D
+    assert rows16(base[:n].view(T, H, D)).data_ptr() == base.data_ptr()  # taken as it is
+    wide = base[:T * (H * D + 32)].view(T, H * D + 32)
+    fused = wide[:, 16:16 + H * D].view(T, H, D)
+    assert rows16(fused).data_ptr() == fused.data_ptr()
+    for x in (base[1:1 + n].view(T, H, D), wide[:, 3:3 + H * D].view(T, H, D),
+              base[1:1 + n].view(T, D, H).transpose(1, 2)):
+        y = rows16(x)
+        assert y.data_ptr() % 16 == 0 and y.is_contiguous()
+        assert torch.equal(y.view(torch.uint8), torch.stack(list(x)).contiguous().view(torch.uint8))  # (values may be NaN)
