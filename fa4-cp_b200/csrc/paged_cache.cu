@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanParams 
 constexpr int kMaskThreads = 256;
 constexpr int kMaxNodes = 4096;  // parents of one tree in shared memory (16 KB)
 
-// One CTA per (request, share of its words); CTA nseq clears the rows outside every request.
+// One CTA per (request, share of its words); CTA nseq clears the rows before the first request and
+// behind the last.  A tree whose bounds leave the rows is no tree: the rows between them are cleared.
 // A thread owns one 64-bit word of one node and walks the node's ancestors in shared memory
 // (parents come before children, so the walk descends and ends at the word's first bit).  1.8 us
 // for 8 trees of 8 nodes (the launch), 4.4 us for 512 of 200 (the walks; 3.3 MB written).
@@ -230,7 +231,14 @@ __global__ void __launch_bounds__(kMaskThreads)
     return;
   }
   const int64_t a = cu[j], b = cu[j + 1];
-  if (a < 0 || b > total || b <= a) return;
+  if (a < 0 || b > total) {
+    const int64_t lo = max(a, int64_t(0)) * words, hi = min(b, total) * words;
+    for (int64_t i = lo + int64_t(blockIdx.y) * kMaskThreads + threadIdx.x; i < hi;
+         i += int64_t(gridDim.y) * kMaskThreads)
+      mask[i] = 0;
+    return;
+  }
+  if (b <= a) return;
   const int n = int(min(b - a, int64_t(max_nodes)));
   for (int i = threadIdx.x; i < n; i += kMaskThreads) {
     const int par = parents[a + i];

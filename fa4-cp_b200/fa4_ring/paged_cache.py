@@ -117,8 +117,9 @@ def paged_tree_mask(parents: torch.Tensor, cu_seqlens_q: torch.Tensor, *,
     ``parents`` (int32 ``[T]``): for each node the index of its parent within its own tree, -1
     for a child of the last cached token.  Parents come before their children; a parent that
     does not (or a negative one) counts as none.  ``cu_seqlens_q`` (int32 ``[nseq + 1]``)
-    bounds the trees; ``max_nodes`` (at most 4096) bounds their sizes.  Rows outside every
-    tree are 0.  Built once a step, used by every layer."""
+    bounds the trees, ascending; ``max_nodes`` (at most 4096) bounds their sizes.  Rows outside
+    every tree are 0, and so are those of a tree whose bounds leave the rows.  Built once a step,
+    used by every layer."""
     _lib.require_cuda(parents)
     dev = parents.device
     assert parents.dim() == 1 and cu_seqlens_q.dim() == 1, "parents is [T], cu_seqlens_q [nseq + 1]"

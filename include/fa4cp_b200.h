@@ -542,7 +542,9 @@ FA4CP_API int fa4cp_add_f32(float* dst, const float* src, int64_t n, void* strea
  * fa4cp_paged_tree_mask: mask int64 [total_q, ceil(max_nodes / 64)], bit m of word w of row
  *   cu_q[j] + i: node i of tree j sees node 64 w + m (itself and its ancestors).  parents
  *   int32 [total_q]: the parent's index in its tree, below the child's; anything else: none.
- *   Rows outside every tree are 0.  max_nodes <= 4096.
+ *   Rows outside every tree are 0, and so are those of a tree whose bounds leave [0, total_q)
+ *   (bounds ascend: where they do not, the bits of the rows between them are unspecified).
+ *   max_nodes <= 4096.
  *
  * fa4cp_paged_kv_write: rows k, v [num_tokens, Hkv, D] at token strides (elements, 16-byte
  *   aligned) into the pools at slot_mapping; slots outside [0, num_pages * page_size) are

@@ -153,3 +153,26 @@ def test_unaligned_rows_of_one_token():
         paged_kv_write(k, v, pools[0], pools[1], slots)
         assert torch.equal(pools.view(2, 32, 2, 128)[:, 5:5 + T], rows)
     assert_device_ok()
+
+
+@pytest.mark.parametrize("cu,total", [([0, 4, 14], 10), ([0, 14], 10), ([-3, 2, 6], 9), ([12, 14], 10),
+                                      ([-9, -2], 5), ([0, 3, 3, 8, 2 ** 31 - 1], 11), ([-2 ** 31, 2, 5], 7)])
+@pytest.mark.parametrize("nodes", [16, 130])
+def test_tree_mask_bounds_past_the_rows(cu, total, nodes):
+    """A tree whose bounds leave the rows is no tree: its rows are 0, as those outside every tree,
+    and the trees beside it are whole."""
+    from fa4_ring import _lib
+    words = (nodes + 63) // 64
+    parents = torch.tensor([(i % 3) - 1 for i in range(total)], dtype=torch.int32)
+    mask = torch.full((total + 2, words), -1, dtype=torch.int64, device="cuda")
+    par, bounds = parents.cuda(), i32(cu)
+    rc = _lib.load().fa4cp_paged_tree_mask(par.data_ptr(), bounds.data_ptr(), len(cu) - 1, total, nodes,
+                                           mask.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0
+    want_mask = torch.zeros(total, words, dtype=torch.int64)
+    for j, (a, b) in enumerate(zip(cu, cu[1:])):
+        if 0 <= a < b <= total:
+            want_mask[a:b] = ph.pack(ph.seen_of(parents, cu, j), words)
+    assert torch.equal(mask[:total].cpu(), want_mask)
+    assert bool((mask[total:] == -1).all())
