@@ -53,7 +53,11 @@ def norm_descale(d: Optional[torch.Tensor], h_kv: int, device) -> Optional[torch
             and d.device == device and d.is_contiguous()):
         return d
     if not torch.is_tensor(d):
-        d = torch.tensor(float(d))
+        return torch.full((h_kv,), float(d), dtype=torch.float32, device=device)
+    if not d.is_cuda and (d.dim() == 0 or d.numel() == h_kv == 1):
+        # one number on the host is filled in on the device: a copy of it would wait for the
+        # stream, and could not be captured into a graph
+        return torch.full((h_kv,), d.detach().item(), dtype=torch.float32, device=device)
     d = d.to(device=device, dtype=torch.float32)
     if d.dim() == 0:
         d = d.reshape(1).expand(h_kv)
@@ -269,6 +273,8 @@ def rows16(x: torch.Tensor) -> torch.Tensor:
 
 
 def as_i32(t: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """``t`` as dense int32 on ``dev``, itself if it is that.  A tensor on the host is copied, which
+    waits for the stream and cannot be captured into a graph."""
     if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
         return t
     return t.to(device=dev, dtype=torch.int32).contiguous()
@@ -310,7 +316,9 @@ def b200_attn_paged_tree(
     over the GPU whatever the batch.  Returns ``(out [T, H, D], lse [T, H] fp32 natural log)``;
     out has q's dtype (bf16 for e4m3).  A row that sees no key gets out 0, lse -inf.  What lies
     behind ``seq_lens`` in a page never reaches the result, nor does what a token does not see.
-    Rows outside ``cu_seqlens_q`` are left unwritten."""
+    Rows outside ``cu_seqlens_q`` are left unwritten.  ``cu_seqlens_q``, ``seq_lens`` or descales of
+    several heads that are on the host are copied to q's device, which waits for the stream and
+    cannot be captured into a graph."""
     _lib.require_cuda(q, k_pages, v_pages, block_table, tree_mask)
     assert q.dim() == 3, "expected a [T, H, D] q"
     assert k_pages.dim() == 4 and k_pages.shape == v_pages.shape, "pools are [pages, page, H_kv, D]"

@@ -17,9 +17,11 @@ The pools are ``[num_pages, page_size, H_kv, D]``; logical row ``r`` of request 
     cached_lens = paged_kv_accept(k_pages, v_pages, plan.block_table, cached_lens, accepted,
                                   cu_seqlens_q=plan.cu_seqlens_q)
 
-Nothing here copies to the host, waits for the GPU or validates device data: lengths, slots
-and tables are read by the kernels, which keep every access inside the tensors that they were
-given.  Every call can be captured into a CUDA graph.
+Nothing here copies to the host or validates device data: lengths, slots and tables are read by
+the kernels, which keep every access inside the tensors that they were given.  With its tensors on
+the device (a descale may also be a number) no call waits for the GPU, and every one can be
+captured into a CUDA graph.  ``cu_seqlens_q``, ``seq_lens`` and descales of several heads are also
+taken from the host; copying those waits for the stream and cannot be captured.
 """
 
 from typing import NamedTuple, Optional

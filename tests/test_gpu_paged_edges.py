@@ -176,3 +176,35 @@ def test_tree_mask_bounds_past_the_rows(cu, total, nodes):
             want_mask[a:b] = ph.pack(ph.seen_of(parents, cu, j), words)
     assert torch.equal(mask[:total].cpu(), want_mask)
     assert bool((mask[total:] == -1).all())
+
+
+@pytest.mark.parametrize("number", [0.02, torch.tensor(0.02), torch.tensor([[0.02]]), torch.tensor([0.02])],
+                         ids=["float", "0-d", "1x1", "1"])
+def test_capture_with_descales_on_the_host(number):
+    """A descale that is one number, wherever it is, is no copy from the host: the calls can be
+    captured into a graph, and give what a descale on the device gives."""
+    from fa4_ring import b200_attn_paged_tree, paged_kv_write
+    x = make([40, 9], [2, 1], 4, 1, 128, BF, E4M3, 16, seed=41, tree=False)
+    x["kd"] = x["vd"] = torch.tensor([0.02])
+    ref = call(x)
+    q, k, v, tb, cu = (dev(x[n]) for n in ("q", "k", "v", "table", "cu"))
+    lens = i32(x["lens"])
+    rows = torch.randn(3, 1, 128, generator=torch.Generator().manual_seed(2)).to(BF).cuda()
+    slots = torch.tensor([1, 5, 17]).cuda()
+    pools = torch.zeros(4, 2, 16, 1, 128, dtype=E4M3, device="cuda")
+    paged_kv_write(rows, rows, pools[0], pools[1], slots, k_descale=dev(x["kd"]), v_descale=dev(x["kd"]))
+
+    def step():
+        paged_kv_write(rows, rows, pools[2], pools[3], slots, k_descale=number, v_descale=number)
+        return b200_attn_paged_tree(q, k, v, tb, cu_seqlens_q=cu, seq_lens=lens, max_seqlen_q=2,
+                                    k_descale=number, v_descale=number)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out, lse = step()
+    pools.view(torch.uint8)[2:] = 0
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref[0]) and torch.equal(lse, ref[1])
+    assert torch.equal(pools[2].view(torch.uint8), pools[0].view(torch.uint8))
+    assert torch.equal(pools[3].view(torch.uint8), pools[1].view(torch.uint8))
+    assert_device_ok()

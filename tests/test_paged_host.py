@@ -28,3 +28,21 @@ def test_rows_end_up_aligned(dt, T, H, D):
         y = rows16(x)
         assert y.data_ptr() % 16 == 0 and y.is_contiguous()
         assert torch.equal(y.view(torch.uint8), torch.stack(list(x)).contiguous().view(torch.uint8))  # (values may be NaN)
+
+
+@pytest.mark.parametrize("h_kv", [1, 3])
+def test_descales_of_every_form(h_kv):
+    from fa4_ring.attn_backend import norm_descale
+    dev = torch.device("cpu")
+    assert norm_descale(None, h_kv, dev) is None
+    for d in (0.3, torch.tensor(0.3), torch.tensor(0.3, dtype=torch.float64, requires_grad=True),
+              torch.full((1, h_kv), 0.3), torch.full((h_kv,), 0.3, dtype=torch.float64)):
+        got = norm_descale(d, h_kv, dev)
+        assert got.dtype == torch.float32 and got.is_contiguous() and not got.requires_grad
+        assert got.flatten().tolist() == torch.full((h_kv,), 0.3).tolist()
+    for d in (torch.ones(h_kv + 1), torch.ones(1, h_kv + 1)):
+        with pytest.raises(AssertionError):
+            norm_descale(d, h_kv, dev)
+    if h_kv > 1:
+        with pytest.raises(AssertionError):  # one entry is not a scalar
+            norm_descale(torch.ones(1), h_kv, dev)
