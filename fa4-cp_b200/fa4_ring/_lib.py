@@ -179,9 +179,19 @@ def dtype_code(dt: torch.dtype) -> int:
         raise ValueError(f"unsupported dtype {dt}") from None
 
 
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The handle alone and the device's index without the checks around it: a torch.cuda.Stream object
+# costs 2 us, as much as the launch.  Both calls are torch's own, so a torch without them is served
+# by the public ones.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _public_stream
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def stream_of(t: torch.Tensor) -> int:
-    # the handle alone: a torch.cuda.Stream object costs 2 us, as much as the launch
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    return _raw_stream(t.get_device())
 
 
 _no_switch = contextlib.nullcontext()
@@ -189,7 +199,7 @@ _no_switch = contextlib.nullcontext()
 
 def on_device(dev: torch.device):
     """Context in which launches go to ``dev`` (nothing to do when it is the current device)."""
-    return _no_switch if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+    return _no_switch if dev.index == _current_device() else torch.cuda.device(dev)
 
 
 def ptr(t) -> int:

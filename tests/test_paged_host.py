@@ -46,3 +46,38 @@ def test_descales_of_every_form(h_kv):
     if h_kv > 1:
         with pytest.raises(AssertionError):  # one entry is not a scalar
             norm_descale(torch.ones(1), h_kv, dev)
+
+
+def test_launch_stream_and_device_without_the_private_calls(monkeypatch):
+    """The stream and the device of a launch come from torch's private calls, which are the cheaper
+    ones; a torch without them is served by the public ones."""
+    import importlib
+
+    from fa4_ring import _lib
+
+    class Stream:
+        def __init__(self, index):
+            self.cuda_stream = 1000 + index
+
+    class Tensor:
+        def get_device(self):
+            return 3
+
+    try:
+        with monkeypatch.context() as m:
+            m.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+            m.delattr(torch._C, "_cuda_getDevice", raising=False)
+            m.setattr(torch.cuda, "current_stream", Stream)
+            m.setattr(torch.cuda, "current_device", lambda: 3)
+            importlib.reload(_lib)
+            assert _lib.stream_of(Tensor()) == 1003
+            assert _lib.on_device(torch.device("cuda", 3)) is _lib._no_switch
+            assert isinstance(_lib.on_device(torch.device("cuda", 2)), torch.cuda.device)
+        with monkeypatch.context() as m:
+            m.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 2000 + i, raising=False)
+            m.setattr(torch._C, "_cuda_getDevice", lambda: 1, raising=False)
+            importlib.reload(_lib)
+            assert _lib.stream_of(Tensor()) == 2003
+            assert _lib.on_device(torch.device("cuda", 1)) is _lib._no_switch
+    finally:
+        importlib.reload(_lib)
