@@ -1323,19 +1323,6 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeParams p) {
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-int sm_count(int* out) {
-  static std::atomic<int> cached{0};
-  int n = cached.load();
-  if (n == 0) {
-    int dev = 0;
-    FA4CP_CHECK_CUDA(cudaGetDevice(&dev));
-    FA4CP_CHECK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    cached.store(n);
-  }
-  *out = n;
-  return FA4CP_OK;
-}
-
 constexpr int kMaxGrid = 148;  // B200's SMs: sizes the workspace without a device
 
 int64_t workspace_bytes_for(int D) {
@@ -1393,7 +1380,7 @@ int launch_tree(const void* k_pages, const void* v_pages, const int64_t* ks, con
     optin.fetch_or(bit);
   }
   int sms = 0;
-  if (int rc = sm_count(&sms)) return rc;
+  FA4CP_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   const int grid = sms < kMaxGrid ? sms : kMaxGrid;
   const int rows = p.page_size < TR::BN ? p.page_size : TR::BN;
   const int el = TR::KV8 ? 1 : 2;

@@ -47,3 +47,12 @@ def test_no_lane_leaves_a_loop_of_warp_collective_accesses():
         for cond, jump in _jumps(body):
             names = set(re.findall(r"[A-Za-z_]\w*", cond))
             assert not names & PER_LANE, f"`if ({cond}) {jump}` parts the lanes of a warp"
+
+
+def test_the_grid_is_of_the_device_of_the_call():
+    """The number of SMs is asked of the device that the call runs on, not kept from the first one."""
+    text = re.sub(r"//[^\n]*", "", open(SRC).read())
+    at = text.index("int launch_tree(")
+    body = text[text.index("{", at):_close(text, text.index("{", at), "{}")]
+    assert "cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)" in body
+    assert text.count("MultiProcessorCount") == 1
