@@ -208,3 +208,12 @@ def test_capture_with_descales_on_the_host(number):
     assert torch.equal(pools[2].view(torch.uint8), pools[0].view(torch.uint8))
     assert torch.equal(pools[3].view(torch.uint8), pools[1].view(torch.uint8))
     assert_device_ok()
+
+
+def test_launches_counted():
+    """The attention is two kernels: the parts, and their join."""
+    from fa4_ring import _lib
+    x = make([40], [2], 4, 1, 128, BF, BF, 16, seed=44)
+    before = _lib.launch_count
+    call(x)
+    assert _lib.launch_count == before + 2
