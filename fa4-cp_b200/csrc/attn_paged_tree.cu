@@ -426,10 +426,11 @@ __device__ __forceinline__ void q16_terms(const uint4 a, const uint4 b, float f,
 // reads V again from the pool.
 template <int D, int STEP>
 __device__ __forceinline__ void add_nonfinite(const TreeParams& p, int seq, int kvh, int ctx, int lim,
-                                              int64_t tok, int node, int key0, int key1, int first,
+                                              int64_t tok, int node, int key0, int64_t key1, int first,
                                               uint16_t* out_row, float* part_row) {
+  const int end = int(min(key1, int64_t(lim)));
 #pragma unroll 1
-  for (int key = max(max(key0, ctx), 0); key < min(key1, lim); ++key) {
+  for (int key = max(max(key0, ctx), 0); key < end; ++key) {
     if (!(seen32(p, ctx, lim, tok, node, key) & 1u)) continue;
     const int e = key / p.page_size;
     const int page = p.block_table[int64_t(seq) * p.max_pages + e];
@@ -1004,7 +1005,8 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
         tc_fence_after();
         const int kbase = (x.kt0 + j) * BN;
-        const bool edge = kbase + BN > ctx || kbase + BN > x.lim;  // new rows, or the cache's end
+        // new rows, or the cache's end (kbase + BN may be 2^31)
+        const bool edge = ctx - kbase < BN || x.lim - kbase < BN;
         const uint32_t t_s = t_lane + uint32_t(TR::TM_S) + it % NB * BN;
         constexpr int C = BN / 32;
         uint32_t vis[C];
@@ -1245,8 +1247,8 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           else __stcg(&p.part_ml[part * BM + t], make_float2(ms, l));
         }
         if (sees_bad)
-          add_nonfinite<D, NWG>(p, x.seq, x.kvh, ctx, x.lim, tok, node, x.kt0 * BN, (x.kt0 + n) * BN, wg, out_row,
-                                whole ? nullptr : prow);
+          add_nonfinite<D, NWG>(p, x.seq, x.kvh, ctx, x.lim, tok, node, x.kt0 * BN, int64_t(x.kt0 + n) * BN, wg,
+                                out_row, whole ? nullptr : prow);
       }
       if (threadIdx.x == 0 && !more && x.kt0 == 0 && !whole) {
         // the share's last item began here and goes on: this CTA's descriptor names it, and the

@@ -217,3 +217,29 @@ def test_launches_counted():
     before = _lib.launch_count
     call(x)
     assert _lib.launch_count == before + 2
+
+
+@pytest.mark.parametrize("q_dt,kv_dt,D,page", [(BF, BF, 64, 256), (BF, E4M3, 128, 128), (F16, F16, 256, 512)])
+@pytest.mark.parametrize("shown", [False, True])
+def test_a_cache_that_ends_at_the_last_int32(q_dt, kv_dt, D, page, shown):
+    """2^31 - 1 cached rows, over a table that names one page again and again: the last tile ends
+    where 32 bits do.  The row behind the cache holds NaN, and so does, if it is shown, the last of two
+    new rows."""
+    from fa4_ring import b200_attn_paged_tree
+    n = 2 ** 31 - 1
+    table = torch.zeros(1, 2 ** 31 // page, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    k = torch.zeros(2, page, 1, D)
+    v = torch.ones(2, page, 1, D)
+    k[1, page - 1], v[1, page - 1] = math.nan, math.nan  # row 2^31 - 1
+    if shown:
+        v[1, page - 2] = math.nan                         # row 2^31 - 2: the second new row
+    q = torch.ones(2, 1, D)
+    out, lse = b200_attn_paged_tree(q.to(q_dt).cuda(), k.to(kv_dt).cuda(), v.to(kv_dt).cuda(), table,
+                                    cu_seqlens_q=i32([0, 2]), seq_lens=i32([n]), max_seqlen_q=2)
+    # all weights are one power of two, so the sums and O are exact until the parts are joined
+    good = out if not shown else out[:1]
+    assert ((good.double() - 1).abs() <= ph.HALF_STEP[q_dt] + 2.0 ** -15).all()
+    assert not shown or out[1].isnan().all()
+    assert (lse.double() - math.log(n)).abs().max().item() <= 2.0 ** -20 + 2.0 ** -22 * math.log(n) + 2.0 ** -16
+    assert_device_ok()
