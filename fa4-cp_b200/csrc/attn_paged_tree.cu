@@ -79,8 +79,13 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units: P <= 256 times the lar
 // which is the output's own rounding.)  An f16 also ends at the bottom: it is subnormal below
 // 2^-14 and 0 below 2^-25, while the sum of the weights is in 32 bits and keeps them all.  So an f16 P
 // carries a factor of 2^7, which the sum and O share: the largest weight is between 2^7 and 2^15, and
-// what is lost of a weight is below 2^-32 of it.
+// what is lost of a weight is below 2^-32 of it.  (It is added to the finished offset: with an fma or a
+// product rounded upwards in its place the warpgroups fall into step at head_dim 64, and e4m3 with one
+// token takes 162 us instead of 140.)
 constexpr float kLiftF16 = 7.0f;
+// An offset of 2^22 and more is off by a quarter and more.  The maximum is raised with every larger one
+// there, so that this and the threshold do not add up past the end of an f16.
+constexpr float kExactBelow = 0x1p22f;
 constexpr int BM = 128;
 
 // codes written to the device status word when a bounded wait gives up
@@ -990,12 +995,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
         scale /= qf;
         scale = scale < 1.17549435e-38f ? 1.17549435e-38f : scale;
       }
-      // What a row's exponents (log2 units) are relative to, given its maximum.  Rounded upwards for
-      // an f16 P, so that no rounding of a large maximum takes P past 2^15; sums and O are brought
-      // from one maximum to another by the difference of these same numbers.
-      auto offset = [&](float mx) -> float {
-        return !TR::KV8 && bf16_op ? mx * scale : __fmaf_ru(mx, scale, -kLiftF16);
-      };
+      const float lift = !TR::KV8 && bf16_op ? 0.f : kLiftF16;
       // m: the maximum that this warpgroup's sum l (and its O) are relative to
       float m = kNegInf, l = 0.f;
       bool sees_bad = false;
@@ -1050,7 +1050,9 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
             if (!max_settled()) { aborted = true; break; }
             if (j > 0) so_far = row_max[t];
           }
-          const bool raise = so_far == kNegInf ? mx != kNegInf : (mx - so_far) * scale > kRescaleThreshold;
+          const bool raise = so_far == kNegInf ? mx != kNegInf
+                                               : (mx - so_far) * scale >
+                                                     (fabsf(mx) * scale < kExactBelow ? kRescaleThreshold : 0.f);
           const float m_new = raise ? mx : so_far;
           if constexpr (!TR::APART) {
             row_max[t] = m_new;
@@ -1059,12 +1061,12 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
           }
           // from here on off the other warpgroup's way
           if (m_new != m) {
-            if (m != kNegInf) l *= ex2_approx(offset(m) - offset(m_new));
+            if (m != kNegInf) l *= ex2_approx((m - m_new) * scale);
             m = m_new;
           }
           constexpr int MINE = TR::APART ? NWG : 1;  // PV(it - MINE) was the last one into this O
           if (j >= MINE && __any_sync(0xffffffffu, raise)) {
-            const float f = !raise ? 1.f : so_far == kNegInf ? 0.f : ex2_approx(offset(so_far) - offset(m_new));
+            const float f = !raise ? 1.f : so_far == kNegInf ? 0.f : ex2_approx((so_far - m_new) * scale);
             ok = mbar_wait(o_done(it - MINE), phase(it - MINE, NB), abort, kErrODone, status);
             if (!__all_sync(0xffffffffu, ok)) { aborted = true; break; }
             tc_fence_after();
@@ -1080,7 +1082,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
             }
           }
           // (P = 0 in a lane without a row, for the same reason)
-          const float neg_m = !valid ? kNegInf : (m == kNegInf) ? 0.f : -offset(m);
+          const float neg_m = (!valid ? kNegInf : (m == kNegInf) ? 0.f : -m * scale) + lift;
           const uint64_t scale2 = f2pack(scale, scale), negm2 = f2pack(neg_m, neg_m);
           uint64_t rs[2] = {0ull, 0ull};
           uint32_t pw[C][16];
@@ -1186,7 +1188,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
 #pragma unroll
       for (int g = 0; g < NWG; ++g) {
         const float lg = end_sum[(set + g) * BM + t], mg = part_f[g];
-        part_f[g] = mg == m ? 1.f : mg == kNegInf ? 0.f : ex2_approx(offset(mg) - offset(m));
+        part_f[g] = mg == m ? 1.f : mg == kNegInf ? 0.f : ex2_approx((mg - m) * scale);
         l += mg == kNegInf ? lg : lg * part_f[g];  // (NaN sums have no maximum)
         sees_bad |= end_bad[(set + g) * BM + t] != 0;
       }
@@ -1241,7 +1243,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1)
       }
       warp_arrive(o_free);
       if (valid) {
-        const float ms = m == kNegInf ? kNegInf : offset(m);
+        const float ms = m == kNegInf ? kNegInf : __fmul_rn(m, scale) - lift;
         if (wg == 0) {
           if (whole) p.lse[tok * p.Hq + head] = l == 0.f ? kNegInf : (ms + lg2_approx(l)) * kLn2;
           else __stcg(&p.part_ml[part * BM + t], make_float2(ms, l));
