@@ -8,13 +8,15 @@
 // are packed into rows of one 128-row MMA tile (row = token * group + head of the group), and
 // K and V are read once for all of them.
 //
-// Measured (32/8 heads, head_dim 128).  64 decoding requests of 1K to 32K tokens, bf16: 0.68 to
-// 0.72 ms = 6.2 to 6.5 TB/s, the rate of a copy.  32 requests of up to 16K tokens: bf16 with 1, 8
-// and 32 new tokens 180, 190 and 200 us (5.3 to 6.1 TB/s); 64 tokens are two row tiles, 381 us
-// (630 TFLOP/s).  Over an e4m3 cache 1 and 64 tokens take 150 and 336 us: a key tile of a CTA
-// takes 1000 to 1100 cycles whatever its bytes, the round trip of an S buffer (S 430, softmax 1810,
-// P to PV 210, PV 600, next S 370 cycles) over the three buffers that TMEM leaves.  One request of
-// 100 and 8K tokens: 11 and 18 us, mostly launch and start.
+// Measured (32/8 heads, head_dim 128; calls of a captured graph).  64 decoding requests of 1K to 32K
+// tokens, bf16: 0.68 to 0.72 ms = 6.2 to 6.5 TB/s, the rate of a copy.  32 requests of 1K to 16K
+// tokens: bf16 with 1, 8 and 32 new tokens 186, 191 and 206 us (5.6 to 6.1 TB/s); 64 tokens are two
+// row tiles, 383 us (620 TFLOP/s).  Over an e4m3 cache 1, 8, 32 and 64 tokens take 139 to 165, 142 to
+// 166, 169 and 331 us: a key tile of a CTA takes 1000 to 1100 cycles whatever its bytes, the round
+// trip of an S buffer (S 430, softmax 1810, P to PV 210, PV 600, next S 370 cycles) over the three
+// buffers that TMEM leaves beside a Q and two O of this layout.  (One token there, and two requests of
+// 256K tokens at head_dim 256, 143 to 200 us, run at one of two speeds from call to call.)  One
+// request of 100 and 8K tokens: 11 and 17 us, mostly launch and start.
 //
 // Schedule.  The work is the list of all (request, K/V head, row tile, key tile), in that
 // order; every CTA takes an equal share of consecutive key tiles, whatever the lengths are
@@ -74,9 +76,9 @@ namespace {
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr float kRescaleThreshold = 8.0f;  // log2 units: P <= 256 times the largest at its maximum
 // P is rounded to the 16-bit type of the V that it multiplies (f16 for an e4m3 V), by half a step:
-// 2^-8 of each weight in bf16, 2^-11 in f16.  (Both operands of an MMA are of one type; bf16 over a
-// bf16 cache, 64 requests of 1K to 32K tokens: 0.0023 off the 64-bit result, all in 32 bits 0.0017,
-// which is the output's own rounding.)  An f16 also ends at the bottom: it is subnormal below
+// 2^-8 of each weight in bf16, 2^-11 in f16.  (Both operands of an MMA are of one type.  Over a bf16
+// cache, 64 requests of 1K to 32K tokens, the result is 0.0023 off the 64-bit one, in norm; with all in
+// 32 bits 0.0017, which is the output's own rounding.)  An f16 also ends at the bottom: it is subnormal below
 // 2^-14 and 0 below 2^-25, while the sum of the weights is in 32 bits and keeps them all.  So an f16 P
 // carries a factor of 2^7, which the sum and O share: the largest weight is between 2^7 and 2^15, and
 // what is lost of a weight is below 2^-32 of it.  (It is added to the finished offset: with an fma or a

@@ -69,7 +69,7 @@ __device__ __forceinline__ void block_scan3(int64_t (&v)[3], int64_t (&tot)[3], 
 // Every CTA repeats the scans over all requests (in chunks of kPlanThreads), then fills its
 // share of the table and of the slots: one launch with no global hand-over, at the price of
 // re-reading 8 bytes a request per CTA from L2.  Bound by the chain lengths, table row, scans,
-// free pages: 6.9 us for 256 requests with 513 pages each, 5.7 us for 64 prompts of 4096 tokens.
+// free pages: 7.1 us for 256 requests with 513 pages each, 5.9 us for 64 prompts of 4096 tokens.
 __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanParams p) {
   __shared__ int s_cached[kPlanThreads], s_cu[kPlanThreads], s_fm[kPlanThreads],
       s_end[kPlanThreads], s_rank[kPlanThreads];
@@ -215,7 +215,9 @@ constexpr int kMaxNodes = 4096;  // parents of one tree in shared memory (16 KB)
 // behind the last.  A tree whose bounds leave the rows is no tree: the rows between them are cleared.
 // A thread owns one 64-bit word of one node and walks the node's ancestors in shared memory
 // (parents come before children, so the walk descends and ends at the word's first bit).  1.8 us
-// for 8 trees of 8 nodes (the launch), 4.4 us for 512 of 200 (the walks; 3.3 MB written).
+// for 8 trees of 8 nodes (the launch), 4.5 us for 512 of 200 (the walks; 3.3 MB written).  A thread of
+// each word walks the same ancestors, so a chain is the worst: one of 4096 nodes takes 432 us, 8 of
+// 1024 84 us.
 __global__ void __launch_bounds__(kMaskThreads)
     tree_mask_kernel(const int32_t* __restrict__ parents, const int32_t* __restrict__ cu, int nseq,
                      int64_t total, int max_nodes, int words, int64_t* __restrict__ mask) {
@@ -334,7 +336,8 @@ constexpr int kWriteThreads = 256, kWriteBlocks = 4, kWriteBatch = 2;
 // memory: a row's loads do not wait for its slot, which decides on the store alone.  Measured:
 // 65536 rows of 8 heads x 128, bf16 into e4m3, 71.5 us = 5.6 TB/s (62.4 us at the rate of a
 // copy); loads marked as streaming 73.5 us, a thread a token instead of the loop 93 us, batches of
-// 4 at 64 registers (spills) 86 us, at 80 registers (3 blocks) 77 us.  64 rows: 1.7 us, the launch.
+// 4 at 64 registers (spills) 86 us, at 80 registers (3 blocks) 77 us.  The same rows copied into a bf16
+// pool: 93 us = 5.6 TB/s.  64 rows: 2 us, the launch.
 template <int QUANT>
 __global__ void __launch_bounds__(kWriteThreads, kWriteBlocks) kv_write_kernel(const WriteParams p) {
   const int cols = min(p.heads * p.per_head, kWriteThreads);  // of a block
@@ -408,7 +411,7 @@ struct AcceptParams {
 // from and goes to) are worked out once, a thread each; then a thread owns a column of K or of V
 // through all of them.  The list ascends, so node a_i >= i: a batch of loads followed by its
 // stores never overwrites a row that a later batch reads.  Bound by three dependent reads (list,
-// table, rows) and, for many requests, by the rows: with the write of 16384 new rows 18 us for 256
+// table, rows) and, for many requests, by the rows: with the write of 12161 new rows 18 to 20 us for 256
 // requests whose 12 rows move over an e4m3 cache (13.5 us of traffic); 26 us when every thread
 // worked the moves out for itself.
 __global__ void __launch_bounds__(kAcceptThreads) kv_accept_kernel(const AcceptParams p) {

@@ -311,9 +311,12 @@ def b200_attn_paged_tree(
     up to its own (bottom-right causal, as :func:`b200_attn`); one token a request is decode.
 
     q is f16 / bf16 with K/V of its dtype, or bf16 / e4m3 with e4m3 K/V (and their descales,
-    scalar, ``[H_kv]`` or ``(1, H_kv)``); head_dim 64, 128 or 256; page_size 16, 32, 64 or a
-    multiple of 128; ``max_seqlen_q`` bounds the requests' new tokens.  The pools may be views of another layout.  Long caches are split
-    over the GPU whatever the batch.  Returns ``(out [T, H, D], lse [T, H] fp32 natural log)``;
+    scalar, ``[H_kv]`` or ``(1, H_kv)``; an f16 q over e4m3 K/V, which has more bits than the two
+    e4m3 terms that a bf16 q is split into, is refused); head_dim 64, 128 or 256; page_size 16, 32,
+    64 or a multiple of 128; ``max_seqlen_q`` bounds the requests' new tokens.  The pools may be
+    views of another layout.  Long caches are split over the GPU whatever the batch.  The weights
+    are rounded to the 16-bit type of the V that they multiply (f16 for e4m3 V), sums and
+    statistics are in fp32; scores are below 2^26 in log2 units.  Returns ``(out [T, H, D], lse [T, H] fp32 natural log)``;
     out has q's dtype (bf16 for e4m3).  A row that sees no key gets out 0, lse -inf.  What lies
     behind ``seq_lens`` in a page never reaches the result, nor does what a token does not see.
     Rows outside ``cu_seqlens_q`` are left unwritten.  ``cu_seqlens_q``, ``seq_lens`` or descales of

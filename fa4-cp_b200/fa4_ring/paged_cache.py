@@ -145,8 +145,9 @@ def paged_kv_write(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor,
 
     Pools of the rows' dtype take copies; e4m3 pools take f16 / bf16 rows as
     ``e4m3(clamp(x / descale))`` with the descales (scalar, ``[H_kv]`` or ``(1, H_kv)``) that
-    the attention multiplies back (``None``: 1).  Tokens with a slot outside the pools (-1)
-    are skipped.  Slots must differ: two tokens with one slot leave a mixture of their rows."""
+    the attention multiplies back (``None``: 1); the attention reads an e4m3 cache under a bf16 or
+    e4m3 q, whichever type the rows came from.  Tokens with a slot outside the pools (-1) are
+    skipped.  Slots must differ: two tokens with one slot leave a mixture of their rows."""
     _check_pools(k_pages, v_pages, k, v, slot_mapping)
     num_pages, page_size, h_kv, d = k_pages.shape
     assert k.dim() == 3 and k.shape == v.shape and k.dtype == v.dtype, "k and v are [T, H_kv, D]"

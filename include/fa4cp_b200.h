@@ -600,7 +600,8 @@ FA4CP_API int fa4cp_paged_kv_accept(void* k_pages, void* v_pages, const int64_t*
  *   workspace    fa4cp_attn_paged_tree_workspace_bytes(...) bytes of scratch, 16-byte aligned
  *                (contents on entry do not matter; calls sharing it must not overlap)
  * Rows behind seq_lens and rows that a token does not see never reach its result, whatever
- * they hold.  Supported: head_dim 64, 128, 256.
+ * they hold.  Supported: head_dim 64, 128, 256; scores below 2^26 in log2 units (the weights'
+ * exponents are fp32, and past it their rounding passes what an f16 or a sum holds).
  */
 FA4CP_API int64_t fa4cp_attn_paged_tree_workspace_bytes(int32_t num_heads_q, int32_t num_heads_kv,
                                                         int32_t head_dim, int32_t max_seqlen_q);
