@@ -243,3 +243,60 @@ def test_a_cache_that_ends_at_the_last_int32(q_dt, kv_dt, D, page, shown):
     assert not shown or out[1].isnan().all()
     assert (lse.double() - math.log(n)).abs().max().item() <= 2.0 ** -20 + 2.0 ** -22 * math.log(n) + 2.0 ** -16
     assert_device_ok()
+
+
+@pytest.mark.parametrize("kv_dt", [BF, E4M3])
+def test_a_whole_step_captured(kv_dt):
+    """Plan, mask, write, attention and accept as one graph, replayed with other lengths, trees and
+    paths (requests of no tokens and of one among them): what the calls give one by one."""
+    from fa4_ring import (b200_attn_paged_tree, paged_block_tables, paged_kv_accept, paged_kv_write,
+                          paged_tree_mask)
+    g = torch.Generator().manual_seed(51)
+    B, H, hk, D, page, width, T = 3, 8, 2, 128, 16, 20, 24
+    desc = dict(k_descale=0.02, v_descale=torch.tensor(0.02)) if kv_dt == E4M3 else {}
+    table = torch.randperm(B * width, generator=g, dtype=torch.int32).view(B, width).clone()
+    table[:, 15:] = -1
+    owned = set(table[:, :15].flatten().tolist())
+    free = [p for p in range(B * width) if p not in owned]
+    fixed = dict(table=table.cuda(), free=i32(free))
+    state = dict(cached=i32([0] * B), new=i32([0] * B), parents=i32([0] * T), accepted=i32([[-1] * 4] * B))
+    pools0 = [(torch.randn(B * width, page, hk, D, generator=g) * 40).to(kv_dt).cuda() for _ in range(2)]
+    x = [torch.randn(T, h, D, generator=g).to(BF).cuda() for h in (H, hk, hk)]
+
+    def step(pools):
+        plan = paged_block_tables(state["cached"], state["new"], fixed["free"], page_size=page, num_tokens=T,
+                                  block_table=fixed["table"])
+        mask = paged_tree_mask(state["parents"], plan.cu_seqlens_q, max_nodes=T)
+        paged_kv_write(x[1], x[2], pools[0], pools[1], plan.slot_mapping, **desc)
+        out, lse = b200_attn_paged_tree(x[0], pools[0], pools[1], plan.block_table, cu_seqlens_q=plan.cu_seqlens_q,
+                                        seq_lens=plan.seq_lens, max_seqlen_q=T, tree_mask=mask, **desc)
+        lens = paged_kv_accept(pools[0], pools[1], plan.block_table, state["cached"], state["accepted"],
+                               cu_seqlens_q=plan.cu_seqlens_q)
+        return plan, mask, out, lse, lens
+
+    ours = [p.clone() for p in pools0]
+    step(ours)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got = step(ours)
+    for cached, new in (([230, 7, 100], [12, 1, 11]), ([0, 239, 240], [1, 0, 9]), ([64, 1, 3], [8, 8, 8])):
+        state["cached"].copy_(i32(cached))
+        state["new"].copy_(i32(new))
+        par = ph.random_parents(new, g)
+        state["parents"].fill_(-1)
+        state["parents"][:par.numel()].copy_(par)
+        state["accepted"].copy_(torch.randint(-1, 9, (B, 4), generator=g).sort(1).values.int())
+        for p, q in zip(ours, pools0):
+            p.view(torch.uint8).copy_(q.view(torch.uint8))
+        gr.replay()
+        torch.cuda.synchronize()
+        theirs = [p.clone() for p in pools0]
+        want_step = step(theirs)
+        n = sum(new)
+        for a, b in zip(got[0], want_step[0]):
+            assert torch.equal(a, b)
+        assert torch.equal(got[1], want_step[1]) and torch.equal(got[4], want_step[4])
+        assert torch.equal(got[2][:n], want_step[2][:n]) and torch.equal(got[3][:n], want_step[3][:n])
+        for a, b in zip(ours, theirs):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert_device_ok()
